@@ -769,6 +769,27 @@ ssmi_status ssmi_expand_merge_bwd_through(const ssmi_expand_desc* d, const void*
 size_t ssmi_expand_weight_partial_bytes(const ssmi_expand_desc* d);
 ssmi_status ssmi_expand_weight_reduce(const ssmi_expand_desc* d, const float* wpart, float* dw, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * 8-bit activation checkpoints: a tensor that waits for the backward pass in one byte per value.
+ * The channels of every pixel are taken in groups of 32 (the last one may be shorter): scales[npix][ceil(c/32)] holds one
+ * biased exponent b per group (the power of two s = 2^(b-127), never under 2^-111), codes[npix][c] the values as e4m3
+ * (OCP FP8, largest 448).  s is the smallest such power of two with max |x| <= 464 s, x / s is rounded to nearest even, and
+ * the restored value code * s is exact in float32 and bfloat16: off by at most half a step, max(|x| 2^-4, s 2^-10).
+ * A group that holds an infinity or a NaN has b = 255 and restores as NaN.
+ *   ssmi_act8_store           x [npix, c] (pixel stride ld, type dtype) -> codes, scales
+ *   ssmi_act8_restore         codes, scales -> y [npix, c] (pixel stride ld_y)
+ *   ssmi_act8_restore_bn_act  for the raw output of a convolution in front of BatchNormalization -> activation ->
+ *                             SpatialDropout: the restored tensor y (nullable) and out = drop * act(bn(y)), the block's output,
+ *                             in one pass (the arithmetic of ssmi_bn_act_drop_fwd on the unrounded restored value; drop [n, c] or
+ *                             NULL, hw pixels per image).  Both are what the block's backward pass reads.
+ * Tensors may be larger than 2 GiB (64-bit offsets).  No counterpart in the reference, which keeps every activation. */
+ssmi_status ssmi_act8_store(const void* x, int64_t ld, int64_t npix, int32_t c, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream);
+ssmi_status ssmi_act8_restore(const uint8_t* codes, const uint8_t* scales, int64_t npix, int32_t c, int32_t dtype, void* y, int64_t ld_y,
+                              void* stream);
+ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales, int64_t npix, int32_t c, int32_t dtype,
+                                     const ssmi_bn_params* bn, int32_t act, const float* alpha, float slope, const float* drop, int64_t hw,
+                                     void* y, int64_t ld_y, void* out, int64_t ld_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -172,6 +172,9 @@ _PROTOS = {
     "ssmi_predict_prepare": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "ssmi_predict_accumulate": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp]),
     "ssmi_predict_topk": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "ssmi_act8_store": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "ssmi_act8_restore": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "ssmi_act8_restore_bn_act": (_i32, [_vp, _vp, _i64, _i32, _i32, _PB, _i32, _vp, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "ssmi_profile_bracket_overhead_ms": (_f32, []),
     "ssmi_device_timestamp": (_i32, [_vp, _vp]),
     "ssmi_device_timestamp_khz": (_i32, []),

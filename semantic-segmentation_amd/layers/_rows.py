@@ -1,0 +1,68 @@
+"""What the row operators (layers.checkpoints, layers.feed_forward, layers.microscaled) share: a tensor's trailing axis is its
+channels, everything in front of it the rows (pixels), and a call runs on the current stream of the tensor's own device."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from .._lib import BF16, F32
+
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+_HERE = contextlib.nullcontext()
+
+
+def dtype_code(t: torch.Tensor, who: str) -> int:
+    try:
+        return _CODES[t.dtype]
+    except KeyError:
+        raise ValueError("{}: float32 or bfloat16 expected, got {}".format(who, t.dtype)) from None
+
+
+def require_gpu(t, who: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("{}: a torch tensor expected, got {}".format(who, type(t).__name__))
+    if not t.is_cuda:      # the error of the pooling layers
+        raise NotImplementedError("{} works only on GPU".format(who))
+
+
+def on(t: torch.Tensor):
+    """The device of `t` as the current one for the length of a call (a no-op where it is)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def rows_of(t: torch.Tensor):
+    """(tensor, rows, row stride): `t` itself where its leading axes step evenly over rows of contiguous channels - a channel
+    slice of a wider tensor, for instance -, a contiguous copy otherwise."""
+    c = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // c if c else 0, c
+    if t.stride(-1) == 1 or c == 1:
+        ld = None
+        step = 1
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if ld is None:
+                ld = stride
+            if stride != ld * step:
+                break
+            step *= size
+        else:
+            if ld is not None and ld >= c:
+                return t, t.numel() // c, ld
+    t = t.contiguous()
+    return t, t.numel() // c if c else 0, c
+
+
+def vector(t, n: int, like: torch.Tensor, who: str, what: str, optional: bool = False):
+    """A float32 vector of n values beside `like`, dense."""
+    if t is None and optional:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != torch.float32 or t.numel() != n:
+        raise ValueError("{}: {} must be {} float32 values on {}".format(who, what, n, like.device))
+    return t.contiguous()
