@@ -790,6 +790,56 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
                                      const ssmi_bn_params* bn, int32_t act, const float* alpha, float slope, const float* drop, int64_t hw,
                                      void* y, int64_t ld_y, void* out, int64_t ld_out, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * Gated feed-forward unit on rows of channels (every pixel of an NHWC tensor is a row):
+ *   y = act(x w_gate + b_gate) * (x w_up + b_up)        x [rows, c] (row stride x_ld), kernels [c, f] (Keras Dense / 1x1), y [rows, f]
+ * act: swish v sigmoid(v), gelu v Phi(v) (exact), relu, sigmoid.  Products of bfloat16 activations take the kernels as bfloat16
+ * (float32 parameters are rounded first); sums are float32.  Biases may both be NULL.
+ * The backward call recomputes both projections from x (nothing else is kept) and overwrites whichever of dx [rows, c] (row
+ * stride x_ld), dw_* [c, f], db_* [f] (parameter type) are not NULL; dy has row stride y_ld.  For bfloat16 the gradients of the
+ * projections are rounded to bfloat16 on their way into the products, and the bias gradients are sums of the rounded ones.
+ * Results are the same on every call (no atomics).  x, w_gate, w_up and ws 16-byte aligned; at most 65536 channels and units and
+ * 2^31 - 1 rows, tensors may pass 2 GiB.  ws: ssmi_gated_ff_workspace_bytes(d, backward) (0 = none; 0 for a refused descriptor too).
+ * Up to 16 rows are answered by a kernel that only streams the kernels.  No counterpart in the reference. */
+enum { SSMI_GATE_SWISH = 0, SSMI_GATE_GELU = 1, SSMI_GATE_RELU = 2, SSMI_GATE_SIGMOID = 3 };
+typedef struct ssmi_gated_desc {
+  int64_t rows, x_ld, y_ld;
+  int32_t c, f;
+  int32_t act;
+  int32_t dtype;         /* x, y and their gradients */
+  int32_t param_dtype;   /* kernels, biases and their gradients: SSMI_F32, or SSMI_BF16 where dtype is SSMI_BF16 */
+} ssmi_gated_desc;
+size_t ssmi_gated_ff_workspace_bytes(const ssmi_gated_desc* d, int32_t backward);
+ssmi_status ssmi_gated_ff_fwd(const ssmi_gated_desc* d, const void* x, const void* w_gate, const void* w_up, const void* b_gate,
+                              const void* b_up, void* y, void* ws, size_t ws_bytes, void* stream);
+ssmi_status ssmi_gated_ff_bwd(const ssmi_gated_desc* d, const void* x, const void* w_gate, const void* w_up, const void* b_gate,
+                              const void* b_up, const void* dy, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* ws,
+                              size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * 4-bit microscaled product for answering: both operands as e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign) with one power of
+ * two per 32 reduction elements (OCP MXFP4), multiplied on the scaled matrix instructions with float32 sums.
+ * Layout of a quantised matrix of `rows` rows along its reduction axis of k: nb = ceil(k / 32) blocks; codes [rows][16 nb] bytes
+ * (element 2 i in the low half of byte i, elements past k are zero), scales [rows][nb] biased exponents.  A block's power of two s
+ * is the smallest one not under 2^-111 with max |x| < 7 s (so the largest value is off by at most half a step), values round to
+ * nearest even.  A block that holds an infinity or a NaN has the exponent 255 and stands for NaNs.
+ *   ssmi_mx4_quantize           x [rows, k] (row stride ld, type dtype) -> codes, scales
+ *   ssmi_mx4_quantize_kernel    a Keras kernel w [k, n] (dense, type dtype) -> codes, scales of its n columns
+ *   ssmi_mx4_dequantize_kernel  codes, scales of n columns -> w [k, n] float32
+ *   ssmi_mx4_dense              y [rows, n] = q(x) w + bias (bias float32 [n] or NULL; y row stride y_ld, type dtype)
+ *   ssmi_mx4_gated              y = act(q(x) w_gate + b_gate) * (q(x) w_up + b_up), SSMI_GATE_* activations
+ * x is quantised inside the product calls (ws: ssmi_mx4_workspace_bytes(rows, k); 16-byte aligned).  codes 16-byte aligned.  At most
+ * 65536 reduction elements and columns and 2^31 - 1 rows; tensors may pass 2 GiB. */
+ssmi_status ssmi_mx4_quantize(const void* x, int64_t ld, int64_t rows, int32_t k, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream);
+ssmi_status ssmi_mx4_quantize_kernel(const void* w, int32_t k, int32_t n, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream);
+ssmi_status ssmi_mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int32_t k, int32_t n, float* w, void* stream);
+size_t ssmi_mx4_workspace_bytes(int64_t rows, int32_t k);
+ssmi_status ssmi_mx4_dense(const void* x, int64_t x_ld, int64_t rows, int32_t k, int32_t n, int32_t dtype, const uint8_t* codes,
+                           const uint8_t* scales, const float* bias, void* y, int64_t y_ld, void* ws, size_t ws_bytes, void* stream);
+ssmi_status ssmi_mx4_gated(const void* x, int64_t x_ld, int64_t rows, int32_t k, int32_t n, int32_t dtype, int32_t act,
+                           const uint8_t* codes_gate, const uint8_t* scales_gate, const uint8_t* codes_up, const uint8_t* scales_up,
+                           const float* b_gate, const float* b_up, void* y, int64_t y_ld, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

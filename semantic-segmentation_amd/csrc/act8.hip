@@ -56,69 +56,72 @@ __device__ __forceinline__ u32x2 load_codes(const uint8_t* p, int n) {
   return w;
 }
 
-// Where a block's work starts: 64 groups a step (four lanes each).  The pixel of the block's first group costs one uniform 64-bit
-// division, the lane's own place in front of it a 32-bit one.
-struct GroupAt {
-  int64_t pix;
-  int g;
+// How a block's 64 lane quartets lie over the tensor: `gp` groups of a pixel side by side (all of them up to 64, then
+// blockIdx.y counts further), `ppb` pixels at a time.  A lane keeps its channels for the whole kernel, so the parameters of its
+// BatchNormalization are loaded once, and walks pixels in steps of the grid.
+struct Lane {
+  int64_t pix, step;      // first pixel, pixels from one step to the next
+  int g, ch, n;           // group, first channel, channels (<= 0: none)
 };
-__device__ __forceinline__ GroupAt group_at(int64_t first, unsigned lane_group, unsigned groups) {
-  const int64_t p0 = first / groups;
-  const unsigned t = (unsigned)(first - p0 * groups) + lane_group;
-  const unsigned dp = t / groups;
-  return {p0 + dp, (int)(t - dp * groups)};
+__device__ __forceinline__ Lane lane_of(int c, int groups) {
+  const int gp = min(groups, 64), ppb = 64 / gp;
+  const int lg = threadIdx.x >> 2, part = threadIdx.x & 3;
+  const int p = lg / gp;
+  Lane l;
+  l.g = lg - p * gp + 64 * (int)blockIdx.y;
+  l.pix = (int64_t)blockIdx.x * ppb + p;
+  l.step = (int64_t)gridDim.x * ppb;
+  l.ch = l.g * kGroup + part * 8;
+  l.n = p < ppb && l.g < groups ? min(8, c - l.ch) : 0;
+  return l;
 }
 
-static constexpr int kSteps = 4;      // groups per lane: independent loads in flight
+static constexpr int kSteps = 4;      // pixels per lane and round: independent loads in flight
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void act8_store_kernel(const T* __restrict__ x, int64_t ld, int64_t ngroups, int c, unsigned groups,
+__global__ __launch_bounds__(256) void act8_store_kernel(const T* __restrict__ x, int64_t ld, int64_t npix, int c, int groups,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int64_t first = (int64_t)blockIdx.x * (64 * kSteps);
-  const unsigned lg = threadIdx.x >> 2, part = threadIdx.x & 3;
-  float v[kSteps][8];
-  int64_t pix[kSteps];
-  int ch[kSteps], n[kSteps], gi[kSteps];
+  const Lane l = lane_of(c, groups);
+  // a block's lanes stay together (the maximum crosses lanes): rounds go by its first pixel
+  for (int64_t base = (int64_t)blockIdx.x * (64 / min(groups, 64)), pix = l.pix; base < npix; base += kSteps * l.step, pix += kSteps * l.step) {
+    float v[kSteps][8];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const GroupAt at = group_at(first, lg + 64 * s, groups);
-    pix[s] = at.pix;
-    gi[s] = at.g;
-    ch[s] = at.g * kGroup + (int)part * 8;
-    n[s] = first + lg + 64 * s < ngroups ? min(8, c - ch[s]) : 0;      // <= 0: nothing here
+    for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
-    if (n[s] > 0) load8<T, VEC>(x + pix[s] * ld + ch[s], n[s], v[s]);
-  }
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(unsigned, v[s][i]) & 0x7FFFFFFFu);
-    top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
-    top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
-    const bool fine = top < 0x7F800000u;
-    // 464 / 256 = 1.8125: a mantissa above it carries into the exponent
-    const int e = max((int)((top + 0x17FFFFu) >> 23) - 8, 16);
-    const float inv = __builtin_bit_cast(float, (unsigned)(254 - (fine ? e : 127)) << 23);
-    u32x2 w = {0u, 0u};
-    if (fine) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k] * inv, v[s][4 * k + 1] * inv, 0, false);
-        w[k] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k + 2] * inv, v[s][4 * k + 3] * inv, q, true);
-      }
+      for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
+      if (l.n > 0 && pix + s * l.step < npix) load8<T, VEC>(x + (pix + s * l.step) * ld + l.ch, l.n, v[s]);
     }
-    if (n[s] > 0) {
-      uint8_t* const d = codes + pix[s] * c + ch[s];
-      if constexpr (VEC) {
-        *reinterpret_cast<u32x2*>(d) = w;
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n[s]) d[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    for (int s = 0; s < kSteps; ++s) {
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(unsigned, v[s][i]) & 0x7FFFFFFFu);
+      top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
+      top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
+      const bool fine = top < 0x7F800000u;
+      // 464 / 256 = 1.8125: a mantissa above it carries into the exponent
+      const int e = max((int)((top + 0x17FFFFu) >> 23) - 8, 16);
+      const float inv = __builtin_bit_cast(float, (unsigned)(254 - (fine ? e : 127)) << 23);
+      u32x2 w = {0u, 0u};
+      if (fine) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k] * inv, v[s][4 * k + 1] * inv, 0, false);
+          w[k] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k + 2] * inv, v[s][4 * k + 3] * inv, q, true);
+        }
       }
-      if (part == 0) scales[pix[s] * groups + gi[s]] = (uint8_t)(fine ? e : 255);
+      const int64_t px = pix + s * l.step;
+      if (l.n > 0 && px < npix) {
+        uint8_t* const d = codes + px * c + l.ch;
+        if constexpr (VEC) {
+          *reinterpret_cast<u32x2*>(d) = w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < l.n) d[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+        }
+        if ((threadIdx.x & 3) == 0) scales[px * groups + l.g] = (uint8_t)(fine ? e : 255);
+      }
     }
   }
 }
@@ -146,61 +149,78 @@ __device__ __forceinline__ void decode8(u32x2 w, unsigned byte, float (&v)[8]) {
 // BN: also the output of the BatchNormalization -> activation -> SpatialDropout behind the stored tensor, which the backward pass
 // needs beside it (operand of the next weight gradient); y (nullable) the restored tensor itself
 template <typename T, bool VEC, bool BN>
-__global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t ngroups, int c,
-                                                           unsigned groups, T* __restrict__ y, int64_t ld_y, RestoreBn bn, T* __restrict__ out,
+__global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t npix, int c,
+                                                           int groups, T* __restrict__ y, int64_t ld_y, RestoreBn bn, T* __restrict__ out,
                                                            int64_t ld_out) {
-  const int64_t first = (int64_t)blockIdx.x * (64 * kSteps);
-  const unsigned lg = threadIdx.x >> 2, part = threadIdx.x & 3;
-  u32x2 w[kSteps];
-  unsigned sc[kSteps];
-  int64_t pix[kSteps];
-  int ch[kSteps], n[kSteps];
+  const Lane l = lane_of(c, groups);
+  if (l.n <= 0) return;
+  float mean[8], invstd[8], gamma[8], beta[8], slope[8];
+  if constexpr (BN) {
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const GroupAt at = group_at(first, lg + 64 * s, groups);
-    pix[s] = at.pix;
-    ch[s] = at.g * kGroup + (int)part * 8;
-    n[s] = first + lg + 64 * s < ngroups ? min(8, c - ch[s]) : 0;
-    w[s] = u32x2{0u, 0u};
-    sc[s] = 127;
-    if (n[s] > 0) {
-      w[s] = load_codes<VEC>(codes + pix[s] * c + ch[s], n[s]);
-      sc[s] = scales[pix[s] * groups + at.g];
+    for (int i = 0; i < 8; ++i) {
+      const int k = min(l.ch + i, c - 1);
+      mean[i] = bn.mean[k];
+      invstd[i] = bn.invstd[k];
+      gamma[i] = bn.gamma[k];
+      beta[i] = bn.beta[k];
+      slope[i] = bn.act == SSMI_ACT_PRELU ? bn.alpha[k] : bn.act == SSMI_ACT_LEAKY ? bn.slope : 1.f;
     }
   }
+  for (int64_t pix = l.pix; pix < npix; pix += kSteps * l.step) {
+    u32x2 w[kSteps];
+    unsigned sc[kSteps];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    if (n[s] <= 0) continue;
-    float v[8];
-    decode8(w[s], sc[s], v);
-    if (!BN || y) store8<T, VEC>(y + pix[s] * ld_y + ch[s], n[s], v);
-    if constexpr (BN) {
-      const float* const drop = bn.drop ? bn.drop + (pix[s] < (1ll << 32) && bn.hw < (1ll << 32) ? (int64_t)((unsigned)pix[s] / (unsigned)bn.hw) : pix[s] / bn.hw) * c
-                                        : nullptr;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = VEC ? ch[s] + i : min(ch[s] + i, c - 1);
-        const float z = bn.gamma[k] * ((v[i] - bn.mean[k]) * bn.invstd[k]) + bn.beta[k];      // the order of bn_act_fwd_kernel
-        const float a = bn.act == SSMI_ACT_PRELU ? bn.alpha[k] : bn.slope;
-        const float r = bn.act == SSMI_ACT_NONE || z > 0.f ? z : a * z;
-        v[i] = drop ? r * drop[k] : r;
+    for (int s = 0; s < kSteps; ++s) {
+      w[s] = u32x2{0u, 0u};
+      sc[s] = 127;
+      if (pix + s * l.step < npix) {
+        w[s] = load_codes<VEC>(codes + (pix + s * l.step) * c + l.ch, l.n);
+        sc[s] = scales[(pix + s * l.step) * groups + l.g];
       }
-      store8<T, VEC>(out + pix[s] * ld_out + ch[s], n[s], v);
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int64_t px = pix + s * l.step;
+      if (px >= npix) break;
+      float v[8];
+      decode8(w[s], sc[s], v);
+      if (!BN || y) store8<T, VEC>(y + px * ld_y + l.ch, l.n, v);
+      if constexpr (BN) {
+        float drop[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) drop[i] = 1.f;
+        if (bn.drop) {
+          const int64_t img = npix <= 0xFFFFFFFFll ? (int64_t)((unsigned)px / (unsigned)bn.hw) : px / bn.hw;      // hw <= npix
+          load8<float, VEC>(bn.drop + img * c + l.ch, l.n, drop);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float z = gamma[i] * ((v[i] - mean[i]) * invstd[i]) + beta[i];      // the order of bn_act_fwd_kernel
+          const float r = z > 0.f ? z : slope[i] * z;
+          v[i] = r * drop[i];
+        }
+        store8<T, VEC>(out + px * ld_out + l.ch, l.n, v);
+      }
     }
   }
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-static ssmi_status check_sizes(const char* who, int64_t npix, int32_t c, int64_t* ngroups) {
-  SSMI_REQUIRE(npix > 0 && c > 0 && c <= (1 << 20), SSMI_E_SHAPE, "%s: %lld pixels of %d channels", who, (long long)npix, c);
-  const int64_t g = (c + kGroup - 1) / kGroup;
-  // one launch holds fewer than 2^32 work-items, four to a group, kSteps groups each
-  SSMI_REQUIRE(npix <= ((1ll << 32) - 256) / g, SSMI_E_UNSUPPORTED, "%s: %lld pixels of %d channels are too many for one launch", who, (long long)npix, c);
-  *ngroups = npix * g;
+static ssmi_status check_sizes(const char* who, int64_t npix, int32_t c) {
+  SSMI_REQUIRE(npix > 0 && npix < (1ll << 48) && c > 0 && c <= (1 << 20), SSMI_E_SHAPE, "%s: %lld pixels of %d channels", who, (long long)npix, c);
   return SSMI_OK;
 }
-static inline dim3 blocks_for(int64_t ngroups) { return dim3((unsigned)ceil_div64(ngroups, 64 * kSteps)); }
+// sixteen rounds of four pixels a lane at the most (the parameters are loaded once per lane), but enough blocks to fill the card
+static inline dim3 blocks_for(int64_t npix, int groups) {
+  const int gp = groups < 64 ? groups : 64, ny = (groups + 63) / 64;
+  const int64_t all = ceil_div64(npix, (int64_t)(64 / gp) * kSteps);
+  int64_t nx = ceil_div64(all, 16);
+  const int64_t fill = ceil_div64(4096, ny);
+  if (nx < fill) nx = all < fill ? all : fill;
+  if (nx > (1 << 20)) nx = 1 << 20;
+  return dim3((unsigned)nx, (unsigned)ny);
+}
 
 }  // namespace ssmi
 
@@ -211,16 +231,15 @@ extern "C" {
 ssmi_status ssmi_act8_store(const void* x, int64_t ld, int64_t npix, int32_t c, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream) {
   SSMI_REQUIRE(x && codes && scales, SSMI_E_INVALID_ARG, "act8_store: null pointer");
   SSMI_REQUIRE(ld >= c, SSMI_E_SHAPE, "act8_store: pixel stride %lld is less than %d channels", (long long)ld, c);
-  int64_t ng;
-  const ssmi_status st = check_sizes("act8_store", npix, c, &ng);
+  const ssmi_status st = check_sizes("act8_store", npix, c);
   if (st != SSMI_OK) return st;
-  const unsigned groups = (unsigned)((c + kGroup - 1) / kGroup);
+  const int groups = (c + kGroup - 1) / kGroup;
   return dispatch_dtype(dtype, [&](auto tag) -> ssmi_status {
     using T = decltype(tag);
     const bool vec = c % 8 == 0 && ld % 8 == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     const T* xt = static_cast<const T*>(x);
-    if (vec) hipLaunchKernelGGL((act8_store_kernel<T, true>), blocks_for(ng), dim3(256), 0, as_stream(stream), xt, ld, ng, c, groups, codes, scales);
-    else hipLaunchKernelGGL((act8_store_kernel<T, false>), blocks_for(ng), dim3(256), 0, as_stream(stream), xt, ld, ng, c, groups, codes, scales);
+    if (vec) hipLaunchKernelGGL((act8_store_kernel<T, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
+    else hipLaunchKernelGGL((act8_store_kernel<T, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
@@ -229,17 +248,16 @@ ssmi_status ssmi_act8_store(const void* x, int64_t ld, int64_t npix, int32_t c, 
 ssmi_status ssmi_act8_restore(const uint8_t* codes, const uint8_t* scales, int64_t npix, int32_t c, int32_t dtype, void* y, int64_t ld_y, void* stream) {
   SSMI_REQUIRE(codes && scales && y, SSMI_E_INVALID_ARG, "act8_restore: null pointer");
   SSMI_REQUIRE(ld_y >= c, SSMI_E_SHAPE, "act8_restore: pixel stride %lld is less than %d channels", (long long)ld_y, c);
-  int64_t ng;
-  const ssmi_status st = check_sizes("act8_restore", npix, c, &ng);
+  const ssmi_status st = check_sizes("act8_restore", npix, c);
   if (st != SSMI_OK) return st;
-  const unsigned groups = (unsigned)((c + kGroup - 1) / kGroup);
+  const int groups = (c + kGroup - 1) / kGroup;
   return dispatch_dtype(dtype, [&](auto tag) -> ssmi_status {
     using T = decltype(tag);
     const bool vec = c % 8 == 0 && ld_y % 8 == 0 && aligned16(y) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     T* yt = static_cast<T*>(y);
     const RestoreBn none = {};
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false>), blocks_for(ng), dim3(256), 0, as_stream(stream), codes, scales, ng, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false>), blocks_for(ng), dim3(256), 0, as_stream(stream), codes, scales, ng, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
@@ -254,17 +272,16 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
   SSMI_REQUIRE(act != SSMI_ACT_PRELU || alpha, SSMI_E_INVALID_ARG, "act8_restore_bn_act: PReLU needs its slopes");
   SSMI_REQUIRE(ld_out >= c && (!y || ld_y >= c), SSMI_E_SHAPE, "act8_restore_bn_act: a pixel stride is less than %d channels", c);
   SSMI_REQUIRE(!drop || (hw > 0 && npix % hw == 0), SSMI_E_SHAPE, "act8_restore_bn_act: %lld pixels are no whole images of %lld", (long long)npix, (long long)hw);
-  int64_t ng;
-  const ssmi_status st = check_sizes("act8_restore_bn_act", npix, c, &ng);
+  const ssmi_status st = check_sizes("act8_restore_bn_act", npix, c);
   if (st != SSMI_OK) return st;
-  const unsigned groups = (unsigned)((c + kGroup - 1) / kGroup);
+  const int groups = (c + kGroup - 1) / kGroup;
   const RestoreBn p = {bn->mean, bn->invstd, bn->gamma, bn->beta, alpha, drop, act, slope, hw};
   return dispatch_dtype(dtype, [&](auto tag) -> ssmi_status {
     using T = decltype(tag);
-    const bool vec = c % 8 == 0 && ld_out % 8 == 0 && aligned16(out) && (!y || (ld_y % 8 == 0 && aligned16(y))) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
+    const bool vec = c % 8 == 0 && ld_out % 8 == 0 && aligned16(out) && (!y || (ld_y % 8 == 0 && aligned16(y))) && (!drop || aligned16(drop)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     T *yt = static_cast<T*>(y), *ot = static_cast<T*>(out);
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true>), blocks_for(ng), dim3(256), 0, as_stream(stream), codes, scales, ng, c, groups, yt, ld_y, p, ot, ld_out);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true>), blocks_for(ng), dim3(256), 0, as_stream(stream), codes, scales, ng, c, groups, yt, ld_y, p, ot, ld_out);
+    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });

@@ -1,0 +1,729 @@
+// Gated feed-forward unit on rows of channels (pixels):
+//   g = x Wg + bg,  u = x Wu + bu,  y = act(g) * u                         x [rows, c], W [c, f] (Keras kernels), y [rows, f]
+// Forward: both projections in one kernel; a wave holds the accumulators of the same 32 units of both, so activation and product
+// happen in registers and g, u never reach memory.
+// Backward: nothing but x is kept.  One kernel recomputes g and u (exact float32 in registers, where storing them would round them to
+// the activation type or double the traffic) and forms in its epilogue, from dy,
+//   dg = dy * u * act'(g),   du = dy * act(g)                              one row [dg | du] per pixel, activation type
+// then  dx = dg Wg^T + du Wu^T  (one product over 2 f) and  dW = x^T dg, x^T du  (one product over the rows, split into strips whose
+// float32 partial sums are added in a fixed order: results do not depend on the launch).
+// All products run on gemm_tile.h: bfloat16 32x32x16 or float32 32x32x2 matrix instructions, float32 sums throughout.
+#include "gemm_tile.h"
+
+namespace ssmi {
+
+enum { kSwish = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
+
+// exp of the bfloat16 variants: v_exp_f32 on x log2(e), relative error under 2^-20 for |x| < 16 - far below the output's 2^-9; the
+// float32 variants take the library's
+template <typename T>
+__device__ __forceinline__ float gate_exp(float v) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(v * 1.44269504f);
+  return expf(v);
+}
+template <typename T>
+__device__ __forceinline__ float gate_sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-v));      // exp = inf gives 0
+}
+template <typename T>
+__device__ __forceinline__ float gate_act(int act, float g) {
+  if (act == kSwish) return g * gate_sigmoid<T>(g);
+  if (act == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678f));
+  if (act == kRelu) return fmaxf(g, 0.f);
+  return gate_sigmoid<T>(g);
+}
+template <typename T>
+__device__ __forceinline__ void gate_act_both(int act, float g, float& a, float& d) {
+  if (act == kSwish) {
+    const float s = gate_sigmoid<T>(g);
+    a = g * s;
+    d = s * (1.f + g * (1.f - s));
+  } else if (act == kGelu) {
+    const float c = 0.5f * (1.f + erff(g * 0.70710678f));
+    a = g * c;
+    d = c + g * 0.39894228f * gate_exp<T>(-0.5f * g * g);
+  } else if (act == kRelu) {
+    a = fmaxf(g, 0.f);
+    d = g > 0.f ? 1.f : 0.f;
+  } else {
+    a = gate_sigmoid<T>(g);
+    d = a * (1.f - a);
+  }
+}
+
+__device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
+  return bf ? (float)static_cast<const bf16*>(p)[i] : static_cast<const float*>(p)[i];
+}
+
+// Which (p, q) tile a workgroup takes.  Consecutive workgroups of an XCD walk kGroupQ row tiles under one column tile, then the
+// next column tile: 32 CUs of an XCD share about eight row tiles and four column tiles through their L2.
+static constexpr int kGroupQ = 8;
+struct TileAt { int p, q; };
+__device__ __forceinline__ TileAt tile_at(unsigned v, unsigned np, unsigned nq) {
+  const unsigned per = kGroupQ * np, grp = v / per, in = v - grp * per;
+  const unsigned gq = min((unsigned)kGroupQ, nq - grp * kGroupQ);
+  return {(int)(in / gq), (int)(grp * kGroupQ + in % gq)};
+}
+
+struct GateArgs {
+  const void *x, *wg, *wu;      // x [rows][x_ld], W [c][w_ld], activation type
+  const void *bg, *bu;          // parameter type or nullptr
+  const void* dy;               // backward
+  void* out;                    // y, or [dg | du]
+  int64_t rows, x_ld, w_ld, out_ld, dy_ld;
+  int c, f, fp;                 // fp: units with the padding that [dg | du] rows have
+  int act, bf_params, vec_out, vec_dy;
+  unsigned np, nq;
+};
+
+template <typename T, int SP, int SQ>
+struct GateSides {
+  static constexpr int kHalf = SP * 32;      // units of a tile
+  typedef Operand<T, kHalf, true> W;
+  typedef Operand<T, SQ * 64, false> X;
+  static constexpr int kStage = 2 * W::kBytes + X::kBytes;
+  W wg, wu;
+  X x;
+  typename W::Reader rw;
+  typename X::Reader rx;
+  int c, wp, wq;
+  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+    const int left = c - t * W::kStepK;
+    wg.request(s, t, left);
+    wu.request(s + W::kBytes, t, left);
+    x.request(s + 2 * W::kBytes, t, left);
+  }
+  __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const {
+    return rw.get(s + (i / (SP / 2)) * W::kBytes, wp * (SP / 2) + i % (SP / 2), ks);
+  }
+  __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + 2 * W::kBytes, wq * SQ + j, ks); }
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4], int n, bool vec) {
+  if (vec && n >= 4) {
+    Act<T>::gst4(p, f32x4{v[0], v[1], v[2], v[3]});
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) Act<T>::gst(p + i, v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void fetch4(const T* p, float (&v)[4], int n, bool vec) {
+  if (vec && n >= 4) {
+    const f32x4 a = Act<T>::gld4(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? Act<T>::gld(p + i) : 0.f;
+  }
+}
+
+template <typename T, int SP, int SQ, bool BWD>
+__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_kernel(GateArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  typedef GateSides<T, SP, SQ> S;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const TileAt at = tile_at(spread_blocks(blockIdx.x, gridDim.x), a.np, a.nq);
+  const int64_t m0 = (int64_t)at.q * (SQ * 64);
+  const int f0 = at.p * S::kHalf;
+  S s;
+  s.c = a.c;
+  s.wp = wave >> 1;
+  s.wq = wave & 1;
+  s.wg.init(static_cast<const T*>(a.wg) + f0, a.w_ld, a.fp - f0);
+  s.wu.init(static_cast<const T*>(a.wu) + f0, a.w_ld, a.fp - f0);
+  s.x.init(static_cast<const T*>(a.x) + m0 * a.x_ld, a.x_ld, (int)min((int64_t)(SQ * 64), a.rows - m0));
+  s.rw.init(lane);
+  s.rx.init(lane);
+  f32x16 acc[SP][SQ];
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.c + S::W::kStepK - 1) / S::W::kStepK, acc);
+
+  const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < SP / 2; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int f = f0 + (s.wp * (SP / 2) + i) * 32 + 8 * k + 4 * hh;
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.bg) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bg[e] = f + e < a.f ? param_at(a.bg, a.bf_params, f + e) : 0.f;
+          bu[e] = f + e < a.f ? param_at(a.bu, a.bf_params, f + e) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < SQ; ++j) {
+        const int64_t m = m0 + (s.wq * SQ + j) * 32 + r;
+        if (m >= a.rows) continue;
+        float o[4];
+        if constexpr (!BWD) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = gate_act<T>(a.act, acc[i][j][4 * k + e] + bg[e]) * (acc[i + SP / 2][j][4 * k + e] + bu[e]);
+          if (f < a.f) store4<T>(static_cast<T*>(a.out) + m * a.out_ld + f, o, a.f - f, a.vec_out);
+        } else {
+          if (f >= a.fp) continue;
+          float dy[4], q[4];
+          fetch4<T>(static_cast<const T*>(a.dy) + m * a.dy_ld + f, dy, a.f - f, a.vec_dy);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u = acc[i + SP / 2][j][4 * k + e] + bu[e];
+            float h, d;
+            gate_act_both<T>(a.act, acc[i][j][4 * k + e] + bg[e], h, d);
+            // padded units have dy = 0, but zero weights times an infinite x are no number: they are set, not multiplied
+            o[e] = f + e < a.f ? dy[e] * u * d : 0.f;
+            q[e] = f + e < a.f ? dy[e] * h : 0.f;
+          }
+          T* const d = static_cast<T*>(a.out) + m * a.out_ld + f;
+          Act<T>::gst4(d, f32x4{o[0], o[1], o[2], o[3]});
+          Act<T>::gst4(d + a.fp, f32x4{q[0], q[1], q[2], q[3]});
+        }
+      }
+    }
+  }
+}
+
+// dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection
+struct GateDxArgs {
+  const void *dgu, *wg, *wu;
+  void* dx;
+  int64_t rows, w_ld, dx_ld;
+  int c, fp, vec_out;
+  unsigned np, nq;
+};
+template <typename T, int SP, int SQ>
+struct DxSides {
+  typedef Operand<T, SP * 64, false> W;
+  typedef Operand<T, SQ * 64, false> D;
+  static constexpr int kStage = W::kBytes + D::kBytes;
+  W wg;
+  D d;
+  __amdgpu_buffer_rsrc_t wu;
+  typename W::Reader rw;
+  typename D::Reader rd;
+  int fp, half, wp, wq;
+  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+    const bool second = t >= half;
+    const int ts = second ? t - half : t, left = fp - ts * W::kStepK;
+    W w = wg;
+    D e = d;
+    if (second) w.rsrc = wu;
+    w.request(s, ts, left);
+    e.request(s + W::kBytes, ts, left, second ? (unsigned)(fp * (int)sizeof(T)) : 0u);
+  }
+  __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rw.get(s, wp * SP + i, ks); }
+  __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rd.get(s + W::kBytes, wq * SQ + j, ks); }
+};
+template <typename T, int SP, int SQ>
+__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dx_kernel(GateDxArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  typedef DxSides<T, SP, SQ> S;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const TileAt at = tile_at(spread_blocks(blockIdx.x, gridDim.x), a.np, a.nq);
+  const int64_t m0 = (int64_t)at.q * (SQ * 64);
+  const int c0 = at.p * (SP * 64);
+  S s;
+  s.fp = a.fp;
+  s.half = (a.fp + S::W::kStepK - 1) / S::W::kStepK;
+  s.wp = wave >> 1;
+  s.wq = wave & 1;
+  s.wg.init(static_cast<const T*>(a.wg) + c0 * a.w_ld, a.w_ld, a.c - c0);
+  s.wu = make_rsrc(static_cast<const T*>(a.wu) + c0 * a.w_ld, 0x7FFFFFFFu);
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (2 * (int64_t)a.fp), 2 * (int64_t)a.fp, (int)min((int64_t)(SQ * 64), a.rows - m0));
+  s.rw.init(lane);
+  s.rd.init(lane);
+  f32x16 acc[SP][SQ];
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, 2 * s.half, acc);
+  const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < SQ; ++j) {
+    const int64_t m = m0 + (s.wq * SQ + j) * 32 + r;
+    if (m >= a.rows) continue;
+    T* const d = static_cast<T*>(a.dx) + m * a.dx_ld;
+#pragma unroll
+    for (int i = 0; i < SP; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + (s.wp * SP + i) * 32 + 8 * k + 4 * hh;
+        const float o[4] = {acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+        if (c < a.c) store4<T>(d + c, o, a.c - c, a.vec_out);
+      }
+  }
+}
+
+// part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]
+struct GateDwArgs {
+  const void *x, *dgu;
+  float* part;
+  int64_t rows, x_ld, strip_rows;
+  int c, cp, fp;                // cp: channels with the padding of x rows
+  unsigned np, nq;
+};
+template <typename T, int SP, int SQ>
+struct DwSides {
+  typedef Operand<T, SP * 64, true> D;
+  typedef Operand<T, SQ * 64, true> X;
+  static constexpr int kStage = D::kBytes + X::kBytes;
+  D d;
+  X x;
+  typename D::Reader rd;
+  typename X::Reader rx;
+  int rows, wp, wq;
+  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+    const int left = rows - t * D::kStepK;
+    d.request(s, t, left);
+    x.request(s + D::kBytes, t, left);
+  }
+  __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rd.get(s, wp * SP + i, ks); }
+  __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + D::kBytes, wq * SQ + j, ks); }
+};
+template <typename T, int SP, int SQ>
+__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dw_kernel(GateDwArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  typedef DwSides<T, SP, SQ> S;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned v = spread_blocks(blockIdx.x, gridDim.x), tiles = a.np * a.nq, strip = v / tiles;
+  const TileAt at = tile_at(v - strip * tiles, a.np, a.nq);
+  const int64_t m0 = (int64_t)strip * a.strip_rows;
+  const int c0 = at.q * (SQ * 64), p0 = at.p * (SP * 64);
+  S s;
+  s.rows = (int)min(a.strip_rows, a.rows - m0);
+  s.wp = wave >> 1;
+  s.wq = wave & 1;
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (2 * (int64_t)a.fp) + p0, 2 * (int64_t)a.fp, 2 * a.fp - p0);
+  s.x.init(static_cast<const T*>(a.x) + m0 * a.x_ld + c0, a.x_ld, a.cp - c0);
+  s.rd.init(lane);
+  s.rx.init(lane);
+  f32x16 acc[SP][SQ];
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, (s.rows + S::D::kStepK - 1) / S::D::kStepK, acc);
+  const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < SQ; ++j) {
+    const int c = c0 + (s.wq * SQ + j) * 32 + r;
+    if (c >= a.c) continue;
+    float* const d = a.part + ((int64_t)strip * a.c + c) * (2 * (int64_t)a.fp);
+#pragma unroll
+    for (int i = 0; i < SP; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = p0 + (s.wp * SP + i) * 32 + 8 * k + 4 * hh;
+        if (p < 2 * a.fp) *reinterpret_cast<f32x4*>(d + p) = f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+      }
+  }
+}
+
+// dW = sum of the strips' partial sums, in their order; four units a thread
+__global__ __launch_bounds__(256) void gate_dw_reduce(const float* __restrict__ part, int strips, int64_t c, int f, int fp, void* dwg, void* dwu, int bf) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // one of c * 2 fp / 4
+  const int quads = fp / 2;
+  if (i >= c * quads) return;
+  const int64_t ci = i / quads;
+  const int p = (int)(i - ci * quads) * 4;
+  const float* s = part + ci * (2 * (int64_t)fp) + p;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  const int64_t step = c * 2 * fp;
+  for (int k = 0; k < strips; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
+  const int fu = p < fp ? p : p - fp;
+  void* const dst = p < fp ? dwg : dwu;
+  if (!dst) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (fu + e < f) {
+      if (bf) static_cast<bf16*>(dst)[ci * f + fu + e] = (bf16)sum[e];
+      else static_cast<float*>(dst)[ci * f + fu + e] = sum[e];
+    }
+}
+
+// column sums of [dg | du]: part[block][2 fp], 4 columns a lane, 64 lanes across, 4 row phases
+template <typename T>
+__global__ __launch_bounds__(256) void gate_db_kernel(const T* __restrict__ dgu, int64_t rows, int64_t strip_rows, int fp, float* __restrict__ part) {
+  __shared__ f32x4 sh[3][64];
+  const int lane = threadIdx.x & 63, ph = threadIdx.x >> 6;
+  const int p = (blockIdx.x * 64 + lane) * 4;
+  const int64_t ld = 2 * (int64_t)fp, m0 = (int64_t)blockIdx.y * strip_rows, m1 = min(rows, m0 + strip_rows);
+  f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+  if (p < 2 * fp) {
+    int64_t m = m0 + ph;
+    for (; m + 4 < m1; m += 8) {
+      s0 += Act<T>::gld4(dgu + m * ld + p);
+      s1 += Act<T>::gld4(dgu + (m + 4) * ld + p);
+    }
+    if (m < m1) s0 += Act<T>::gld4(dgu + m * ld + p);
+  }
+  s0 += s1;
+  if (ph) sh[ph - 1][lane] = s0;
+  __syncthreads();
+  if (!ph && p < 2 * fp) {
+    s0 += sh[0][lane];
+    s0 += sh[1][lane];
+    s0 += sh[2][lane];
+    *reinterpret_cast<f32x4*>(part + blockIdx.y * ld + p) = s0;
+  }
+}
+
+// memory rows brought to the tile engine's form: activation type, rows of cols_p >= cols values (16-byte multiples), zeros behind
+template <typename S, typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const S* __restrict__ src, int64_t ld, int64_t rows, int cols, int cols_p, T* __restrict__ dst) {
+  const int quads = cols_p / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / quads;
+    const int k = (int)(i - r * quads) * 4;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = k + e < cols ? Act<S>::gld(src + r * ld + k + e) : 0.f;
+    Act<T>::gst4(dst + r * cols_p + k, v);
+  }
+}
+
+// A few rows: bound by reading the weights (or by latency), so no tiles and no staging of W.  A workgroup owns 32 units of both
+// projections; 32 threads stand side by side in k for each four units and add their sums at the end.
+template <typename T, typename P, int MB, bool VEC>
+__global__ __launch_bounds__(256) void gate_rows_kernel(GateArgs a) {
+  extern __shared__ float xs[];                     // [MB][c]
+  __shared__ float red[4][8][MB][8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m0 = (int64_t)blockIdx.y * MB;
+  const int nm = (int)min((int64_t)MB, a.rows - m0);
+  for (int i = threadIdx.x; i < MB * a.c; i += 256) {
+    const int m = i / a.c, k = i - m * a.c;
+    xs[i] = m < nm ? Act<T>::gld(static_cast<const T*>(a.x) + (m0 + m) * a.x_ld + k) : 0.f;
+  }
+  __syncthreads();
+  const int quad = lane & 7, slice = wave * 8 + (lane >> 3);
+  const int f = blockIdx.x * 32 + quad * 4;
+  const P *wg = static_cast<const P*>(a.wg) + f, *wu = static_cast<const P*>(a.wu) + f;
+  float sg[MB][4], su[MB][4];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sg[m][e] = su[m][e] = 0.f;
+  const int n = a.f - f;
+  if (n > 0) {
+#pragma unroll 4
+    for (int k = slice; k < a.c; k += 32) {
+      float g[4], u[4];
+      fetch4<P>(wg + (int64_t)k * a.f, g, n, VEC);
+      fetch4<P>(wu + (int64_t)k * a.f, u, n, VEC);
+      if constexpr (sizeof(P) != sizeof(T)) {      // float32 parameters under bfloat16 activations are multiplied as bfloat16
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { g[e] = (float)(T)g[e]; u[e] = (float)(T)u[e]; }
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const float xv = xs[m * a.c + k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sg[m][e] = fmaf(xv, g[e], sg[m][e]);
+          su[m][e] = fmaf(xv, u[e], su[m][e]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int o = 8; o < 64; o <<= 1) {
+        sg[m][e] += __shfl_xor(sg[m][e], o, 64);
+        su[m][e] += __shfl_xor(su[m][e], o, 64);
+      }
+    }
+  if (lane < 8) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        red[wave][lane][m][e] = sg[m][e];
+        red[wave][lane][m][4 + e] = su[m][e];
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nm * 32; i += 256) {
+    const int m = i >> 5, col = i & 31, ff = blockIdx.x * 32 + col;
+    if (ff >= a.f) continue;
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      g += red[w][col >> 2][m][col & 3];
+      u += red[w][col >> 2][m][4 + (col & 3)];
+    }
+    if (a.bg) {
+      g += param_at(a.bg, a.bf_params, ff);
+      u += param_at(a.bu, a.bf_params, ff);
+    }
+    Act<T>::gst(static_cast<T*>(a.out) + (m0 + m) * a.out_ld + ff, gate_act<T>(a.act, g) * u);
+  }
+}
+
+// --------------------------------------------------------------------------------------------------------------- host side
+
+static constexpr int kRowsKernelMost = 16;              // rows that gate_rows_kernel takes (see ssmi_gated_ff_fwd)
+static constexpr int kRowsKernelChannels = 2048;        // its x rows have to fit LDS: 4 x 2048 floats
+
+static inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+struct GatePlan {
+  int es, ce;                       // bytes of an activation, activations in 16 bytes
+  int fp, cp;
+  bool pad_w, pad_x, big_dx, big_dw;
+  int strips;
+  int64_t strip_rows;
+  int db_blocks;
+  int64_t db_rows;
+  size_t w_bytes, x_bytes, dgu_bytes, part_bytes, db_bytes;
+};
+
+static bool wants_big(int64_t rows_q, int64_t cols_p) {
+  // 256 x 256 tiles read LDS half as often per product; they pay from about one round of the 256 CUs on (both sides measured, see
+  // launch_gate), below it the four times as many 128 x 128 tiles finish earlier
+  return ceil_div64(rows_q, 256) * ceil_div64(cols_p, 256) >= 192;
+}
+
+static GatePlan gate_plan(const ssmi_gated_desc* d) {
+  GatePlan p = {};
+  p.es = d->dtype == SSMI_BF16 ? 2 : 4;
+  p.ce = 16 / p.es;
+  p.fp = (int)up_to(d->f, p.ce);
+  p.cp = (int)up_to(d->c, p.ce);
+  p.pad_w = p.fp != d->f || d->param_dtype != d->dtype;
+  p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
+  p.w_bytes = p.pad_w ? 2 * up256((size_t)d->c * p.fp * p.es) : 0;
+  p.x_bytes = p.pad_x ? up256((size_t)d->rows * p.cp * p.es) : 0;
+  p.dgu_bytes = up256((size_t)d->rows * 2 * p.fp * p.es);
+  // strips: about two rounds of workgroups, each strip long enough to be worth its partial sums (512 rows) and short enough that
+  // float32 running sums stay within about 2^-24 sqrt(4096) of exact
+  p.big_dw = (int64_t)ceil_div64(2 * p.fp, 256) * ceil_div64(d->c, 256) * ceil_div64(d->rows, 2048) >= 192;
+  const int64_t side = p.big_dw ? 256 : 128;
+  const int64_t tiles = ceil_div64(2 * p.fp, side) * ceil_div64(d->c, side);
+  int64_t strips = ceil_div64(p.big_dw ? 256 : 512, tiles);
+  strips = strips > ceil_div64(d->rows, 4096) ? strips : ceil_div64(d->rows, 4096);
+  const int64_t most = ceil_div64(d->rows, 512);
+  strips = strips < most ? strips : most;
+  p.strip_rows = up_to(ceil_div64(d->rows, strips), 64);
+  p.strips = (int)ceil_div64(d->rows, p.strip_rows);
+  p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
+  const int64_t dbx = ceil_div64(2 * p.fp, 256);
+  int64_t dby = ceil_div64(1024, dbx);
+  const int64_t dbm = ceil_div64(d->rows, 64);
+  dby = dby < dbm ? dby : dbm;
+  p.db_rows = ceil_div64(d->rows, dby);
+  p.db_blocks = (int)ceil_div64(d->rows, p.db_rows);
+  p.db_bytes = up256((size_t)p.db_blocks * 2 * p.fp * 4);
+  return p;
+}
+
+static ssmi_status check_desc(const char* who, const ssmi_gated_desc* d) {
+  SSMI_REQUIRE(d, SSMI_E_INVALID_ARG, "%s: null descriptor", who);
+  SSMI_REQUIRE(d->rows > 0 && d->c > 0 && d->f > 0, SSMI_E_SHAPE, "%s: %lld rows, %d channels, %d units", who, (long long)d->rows, d->c, d->f);
+  SSMI_REQUIRE(d->c <= 65536 && d->f <= 65536 && d->rows < (1ll << 31), SSMI_E_UNSUPPORTED, "%s: at most 65536 channels and units and 2^31 - 1 rows", who);
+  SSMI_REQUIRE(d->x_ld >= d->c && d->y_ld >= d->f && d->x_ld <= (1 << 20) && d->y_ld <= (1 << 20), SSMI_E_SHAPE,
+               "%s: row strides %lld, %lld under %d channels, %d units (or over 2^20)", who, (long long)d->x_ld, (long long)d->y_ld, d->c, d->f);
+  SSMI_REQUIRE(d->act >= SSMI_GATE_SWISH && d->act <= SSMI_GATE_SIGMOID, SSMI_E_INVALID_ARG, "%s: unknown activation %d", who, d->act);
+  SSMI_REQUIRE(d->dtype == SSMI_F32 || d->dtype == SSMI_BF16, SSMI_E_UNSUPPORTED, "%s: unknown activation dtype %d", who, d->dtype);
+  SSMI_REQUIRE(d->param_dtype == SSMI_F32 || (d->param_dtype == SSMI_BF16 && d->dtype == SSMI_BF16), SSMI_E_UNSUPPORTED,
+               "%s: parameters are float32, or bfloat16 under bfloat16 activations", who);
+  SSMI_REQUIRE((int64_t)d->c * up_to(d->f, 8) * 4 < (1ll << 31), SSMI_E_UNSUPPORTED, "%s: a kernel of 2 GiB or more", who);
+  return SSMI_OK;
+}
+
+static inline bool aligned(const void* p, int b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
+
+template <typename S, typename T>
+static void pad_rows(const void* src, int64_t ld, int64_t rows, int cols, int cols_p, void* dst, hipStream_t st) {
+  const int64_t n = ceil_div64(rows * (cols_p / 4), 256);
+  hipLaunchKernelGGL((pad_rows_kernel<S, T>), dim3((unsigned)(n < 8192 ? n : 8192)), dim3(256), 0, st, static_cast<const S*>(src), ld, rows, cols, cols_p, static_cast<T*>(dst));
+}
+
+// operands in the tile engine's form, padded copies in ws where they are not in it already
+struct Staged {
+  const void *x, *wg, *wu;
+  int64_t x_ld, w_ld;
+  char* ws;      // what is left of the workspace
+};
+template <typename T>
+static Staged stage_operands(const ssmi_gated_desc* d, const GatePlan& p, const void* x, const void* wg, const void* wu, void* ws, hipStream_t st) {
+  Staged s = {x, wg, wu, d->x_ld, d->f, static_cast<char*>(ws)};
+  if (p.pad_w) {
+    const size_t one = p.w_bytes / 2;
+    void *a = s.ws, *b = s.ws + one;
+    if (d->param_dtype == SSMI_BF16) {
+      pad_rows<bf16, T>(wg, d->f, d->c, d->f, p.fp, a, st);
+      pad_rows<bf16, T>(wu, d->f, d->c, d->f, p.fp, b, st);
+    } else {
+      pad_rows<float, T>(wg, d->f, d->c, d->f, p.fp, a, st);
+      pad_rows<float, T>(wu, d->f, d->c, d->f, p.fp, b, st);
+    }
+    s.wg = a;
+    s.wu = b;
+    s.w_ld = p.fp;
+    s.ws += p.w_bytes;
+  }
+  if (p.pad_x) {
+    pad_rows<T, T>(x, d->x_ld, d->rows, d->c, p.cp, s.ws, st);
+    s.x = s.ws;
+    s.x_ld = p.cp;
+    s.ws += p.x_bytes;
+  }
+  return s;
+}
+
+template <typename T, int SP, int SQ, bool BWD>
+static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
+  typedef GateSides<T, SP, SQ> S;
+  a.np = (unsigned)ceil_div64(a.f, S::kHalf);
+  a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
+  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), 2 * S::kStage, st, a);
+  SSMI_LAUNCH_CHECK();
+  return SSMI_OK;
+}
+template <typename T, bool BWD>
+static ssmi_status launch_gate(const GateArgs& a, hipStream_t st) {
+  return wants_big(a.rows, 2 * (int64_t)a.f) ? launch_gate_as<T, 4, 4, BWD>(a, st) : launch_gate_as<T, 2, 2, BWD>(a, st);
+}
+template <typename T, int SP, int SQ>
+static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
+  typedef DxSides<T, SP, SQ> S;
+  a.np = (unsigned)ceil_div64(a.c, SP * 64);
+  a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
+  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), 2 * S::kStage, st, a);
+  SSMI_LAUNCH_CHECK();
+  return SSMI_OK;
+}
+template <typename T, int SP, int SQ>
+static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
+  typedef DwSides<T, SP, SQ> S;
+  a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
+  a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
+  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), 2 * S::kStage, st, a);
+  SSMI_LAUNCH_CHECK();
+  return SSMI_OK;
+}
+
+template <typename T, typename P, int MB>
+static void launch_rows_mb(const GateArgs& a, bool vec, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div64(a.f, 32), (unsigned)ceil_div64(a.rows, MB));
+  const size_t lds = (size_t)MB * a.c * 4;
+  if (vec) hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, true>), grid, dim3(256), lds, st, a);
+  else hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, false>), grid, dim3(256), lds, st, a);
+}
+template <typename T, typename P>
+static ssmi_status launch_rows(const GateArgs& a, hipStream_t st) {
+  const bool vec = a.f % 4 == 0 && aligned(a.wg, 4 * sizeof(P)) && aligned(a.wu, 4 * sizeof(P));
+  if (a.rows == 1) launch_rows_mb<T, P, 1>(a, vec, st);
+  else if (a.rows == 2) launch_rows_mb<T, P, 2>(a, vec, st);
+  else if (a.rows <= 4) launch_rows_mb<T, P, 4>(a, vec, st);
+  else launch_rows_mb<T, P, 4>(a, vec, st);
+  SSMI_LAUNCH_CHECK();
+  return SSMI_OK;
+}
+
+static bool takes_rows_kernel(const ssmi_gated_desc* d) { return d->rows <= kRowsKernelMost && d->c <= kRowsKernelChannels; }
+
+template <typename T>
+static ssmi_status gated_fwd(const ssmi_gated_desc* d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, void* y, void* ws,
+                             hipStream_t st) {
+  GateArgs a = {};
+  a.bg = bg; a.bu = bu; a.out = y; a.out_ld = d->y_ld; a.rows = d->rows; a.c = d->c; a.f = d->f; a.act = d->act;
+  a.bf_params = d->param_dtype == SSMI_BF16;
+  if (takes_rows_kernel(d)) {
+    a.x = x; a.wg = wg; a.wu = wu; a.x_ld = d->x_ld;
+    if (a.bf_params) return launch_rows<T, bf16>(a, st);
+    return launch_rows<T, float>(a, st);
+  }
+  const GatePlan p = gate_plan(d);
+  const Staged s = stage_operands<T>(d, p, x, wg, wu, ws, st);
+  a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.fp = p.fp;
+  a.vec_out = d->y_ld % 4 == 0 && aligned(y, 4 * p.es);
+  return launch_gate<T, false>(a, st);
+}
+
+template <typename T>
+static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dy, void* dx,
+                             void* dwg, void* dwu, void* dbg, void* dbu, void* ws, hipStream_t st) {
+  const GatePlan p = gate_plan(d);
+  Staged s = stage_operands<T>(d, p, x, wg, wu, ws, st);
+  void* const dgu = s.ws;
+  float* const part = reinterpret_cast<float*>(s.ws + p.dgu_bytes);
+  float* const dbp = reinterpret_cast<float*>(s.ws + p.dgu_bytes + p.part_bytes);
+  const int bf = d->param_dtype == SSMI_BF16;
+  GateArgs a = {};
+  a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.bg = bg; a.bu = bu; a.dy = dy; a.out = dgu;
+  a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = 2 * (int64_t)p.fp; a.dy_ld = d->y_ld;
+  a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf;
+  a.vec_dy = d->y_ld % 4 == 0 && aligned(dy, 4 * p.es);
+  ssmi_status r = launch_gate<T, true>(a, st);
+  if (r != SSMI_OK) return r;
+  if (dx) {
+    GateDxArgs b = {};
+    b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp;
+    b.vec_out = d->x_ld % 4 == 0 && aligned(dx, 4 * p.es);
+    r = wants_big(d->rows, d->c) ? launch_dx_as<T, 4, 4>(b, st) : launch_dx_as<T, 2, 2>(b, st);
+    if (r != SSMI_OK) return r;
+  }
+  if (dwg || dwu) {
+    GateDwArgs b = {};
+    b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp;
+    r = p.big_dw ? launch_dw_as<T, 4, 4>(b, p.strips, st) : launch_dw_as<T, 2, 2>(b, p.strips, st);
+    if (r != SSMI_OK) return r;
+    hipLaunchKernelGGL(gate_dw_reduce, dim3((unsigned)ceil_div64((int64_t)d->c * (p.fp / 2), 256)), dim3(256), 0, st, part, p.strips, (int64_t)d->c, d->f, p.fp, dwg, dwu, bf);
+    SSMI_LAUNCH_CHECK();
+  }
+  if (dbg || dbu) {
+    hipLaunchKernelGGL((gate_db_kernel<T>), dim3((unsigned)ceil_div64(2 * p.fp, 256), (unsigned)p.db_blocks), dim3(256), 0, st, static_cast<const T*>(dgu), d->rows, p.db_rows, p.fp, dbp);
+    SSMI_LAUNCH_CHECK();
+    hipLaunchKernelGGL(gate_dw_reduce, dim3((unsigned)ceil_div64(p.fp / 2, 256)), dim3(256), 0, st, dbp, p.db_blocks, (int64_t)1, d->f, p.fp, dbg, dbu, bf);
+    SSMI_LAUNCH_CHECK();
+  }
+  return SSMI_OK;
+}
+
+}  // namespace ssmi
+
+using namespace ssmi;
+
+extern "C" {
+
+size_t ssmi_gated_ff_workspace_bytes(const ssmi_gated_desc* d, int32_t backward) {
+  if (check_desc("gated_ff_workspace_bytes", d) != SSMI_OK) return 0;
+  const GatePlan p = gate_plan(d);
+  if (!backward) return takes_rows_kernel(d) ? 0 : p.w_bytes + p.x_bytes;
+  return p.w_bytes + p.x_bytes + p.dgu_bytes + p.part_bytes + p.db_bytes;
+}
+
+ssmi_status ssmi_gated_ff_fwd(const ssmi_gated_desc* d, const void* x, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* y,
+                              void* ws, size_t ws_bytes, void* stream) {
+  const ssmi_status st = check_desc("gated_ff_fwd", d);
+  if (st != SSMI_OK) return st;
+  SSMI_REQUIRE(x && w_gate && w_up && y, SSMI_E_INVALID_ARG, "gated_ff_fwd: null pointer");
+  SSMI_REQUIRE(!b_gate == !b_up, SSMI_E_INVALID_ARG, "gated_ff_fwd: both biases or none");
+  const size_t need = ssmi_gated_ff_workspace_bytes(d, 0);
+  SSMI_REQUIRE(need == 0 || (ws && ws_bytes >= need), SSMI_E_WORKSPACE, "gated_ff_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  SSMI_REQUIRE(aligned(ws, 16), SSMI_E_INVALID_ARG, "gated_ff_fwd: the workspace must be 16-byte aligned");
+  SSMI_REQUIRE(takes_rows_kernel(d) || ((aligned(x, 16) || gate_plan(d).pad_x) && ((aligned(w_gate, 16) && aligned(w_up, 16)) || gate_plan(d).pad_w)), SSMI_E_INVALID_ARG,
+               "gated_ff_fwd: x and the kernels must be 16-byte aligned");
+  return dispatch_dtype(d->dtype, [&](auto tag) -> ssmi_status { return gated_fwd<decltype(tag)>(d, x, w_gate, w_up, b_gate, b_up, y, ws, as_stream(stream)); });
+}
+
+ssmi_status ssmi_gated_ff_bwd(const ssmi_gated_desc* d, const void* x, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, const void* dy,
+                              void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* ws, size_t ws_bytes, void* stream) {
+  const ssmi_status st = check_desc("gated_ff_bwd", d);
+  if (st != SSMI_OK) return st;
+  SSMI_REQUIRE(x && w_gate && w_up && dy, SSMI_E_INVALID_ARG, "gated_ff_bwd: null pointer");
+  SSMI_REQUIRE(!b_gate == !b_up, SSMI_E_INVALID_ARG, "gated_ff_bwd: both biases or none");
+  const size_t need = ssmi_gated_ff_workspace_bytes(d, 1);
+  SSMI_REQUIRE(ws && ws_bytes >= need, SSMI_E_WORKSPACE, "gated_ff_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  SSMI_REQUIRE(aligned(ws, 16), SSMI_E_INVALID_ARG, "gated_ff_bwd: the workspace must be 16-byte aligned");
+  const GatePlan p = gate_plan(d);
+  SSMI_REQUIRE((aligned(x, 16) || p.pad_x) && ((aligned(w_gate, 16) && aligned(w_up, 16)) || p.pad_w), SSMI_E_INVALID_ARG,
+               "gated_ff_bwd: x and the kernels must be 16-byte aligned");
+  return dispatch_dtype(d->dtype, [&](auto tag) -> ssmi_status {
+    return gated_bwd<decltype(tag)>(d, x, w_gate, w_up, b_gate, b_up, dy, dx, dw_gate, dw_up, db_gate, db_up, ws, as_stream(stream));
+  });
+}
+
+}  // extern "C"

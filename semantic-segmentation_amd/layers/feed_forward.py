@@ -1,0 +1,182 @@
+"""Gated feed-forward unit on the pixels of a channels-last tensor:
+
+    y = act(x w_gate + b_gate) * (x w_up + b_up)
+
+`gated_feed_forward` is the function (differentiable through torch.autograd, its backward pass is HIP kernels too), `GatedFeedForward2D`
+the layer in the manner of the pooling layers.  Parameters are Keras kernels [channels, units] and vectors [units]; float32, or
+bfloat16 under bfloat16 activations.  Nothing but the input waits for the backward pass - in 8 bits with checkpoint="8bit" (the
+gradients are then those at the restored input, layers.checkpoints).  On two MX4Weights (layers.microscaled) the same call answers on
+the 4-bit matrix instructions; that form has no backward pass."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from .._lib import BF16, GatedDesc, lib
+from ._rows import dtype_code, on, require_gpu, rows_of, stream_of
+from .checkpoints import store_8bit
+from .microscaled import MX4Weights, mx4_gated
+
+ACTIVATIONS = {"swish": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _aligned_rows(x):
+    """rows_of with the 16-byte alignment that the products ask of their operands."""
+    t, rows, ld = rows_of(x)
+    if t.data_ptr() % 16:
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+        ld = t.shape[-1]
+    return t, rows, ld
+
+
+def _dense(w):
+    w = w.contiguous()
+    return w.clone() if w.data_ptr() % 16 else w
+
+
+def _workspace(desc, backward, like):
+    n = lib().gated_ff_workspace_bytes(C.byref(desc), backward)
+    return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
+
+
+def _forward(x, wg, wu, bg, bu, act):
+    t, rows, ld = _aligned_rows(x)
+    c, f = wg.shape
+    y = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
+    if not rows:
+        return y
+    d = GatedDesc(rows, ld, f, c, f, act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"))
+    with on(x):
+        ws, n = _workspace(d, 0, x)
+        lib().gated_ff_fwd(C.byref(d), t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), y.data_ptr(), _ptr(ws), n, stream_of(x))
+    return y
+
+
+class _GatedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, bg, bu, act, checkpoint):
+        wg, wu, bg, bu = _dense(wg), _dense(wu), None if bg is None else bg.contiguous(), None if bu is None else bu.contiguous()
+        y = _forward(x, wg, wu, bg, bu, act)
+        ctx.act, ctx.shape, ctx.kept = act, x.shape, None
+        if checkpoint is None or not ctx.needs_input_grad[:5].count(True):
+            ctx.save_for_backward(x, wg, wu, bg, bu)
+        else:
+            ctx.kept = store_8bit(x)
+            ctx.save_for_backward(None, wg, wu, bg, bu)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, bg, bu = ctx.saved_tensors
+        if x is None:
+            x = ctx.kept.restore()
+        need = ctx.needs_input_grad
+        c, f = wg.shape
+        t, rows, ld = _aligned_rows(x)
+        if not rows:
+            return (torch.zeros_like(x) if need[0] else None, *(torch.zeros_like(p) if n else None for p, n in zip((wg, wu, bg, bu), need[1:5])), None, None)
+        if dy.dtype != x.dtype:
+            dy = dy.to(x.dtype)
+        dt, _, dy_ld = rows_of(dy)
+        dx = None
+        if need[0]:      # the row stride of dx is that of x
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            if ld != c:
+                t, ld = _dense(t), c
+        dwg, dwu, dbg, dbu = (torch.empty_like(p) if n else None for p, n in zip((wg, wu, bg, bu), need[1:5]))
+        d = GatedDesc(rows, ld, dy_ld, c, f, ctx.act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"))
+        with on(x):
+            ws, n = _workspace(d, 1, x)
+            lib().gated_ff_bwd(C.byref(d), t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), dt.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu),
+                               _ptr(dbg), _ptr(dbu), _ptr(ws), n, stream_of(x))
+        return dx, dwg, dwu, dbg, dbu, None, None
+
+
+def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="swish", checkpoint=None):
+    """x [..., channels] float32 or bfloat16 on the GPU; w_gate, w_up [channels, units]; b_gate, b_up [units] or both None.
+    activation: "swish", "gelu" (exact), "relu" or "sigmoid".  checkpoint: None, or "8bit" to keep the input in 8 bits for the
+    backward pass.  w_gate and w_up may be MX4Weights (biases then float32): answering on 4-bit products."""
+    who = "gated_feed_forward"
+    require_gpu(x, who)
+    if activation not in ACTIVATIONS:
+        raise ValueError("{}: activation must be one of {}, got {!r}".format(who, sorted(ACTIVATIONS), activation))
+    if checkpoint not in (None, "8bit"):
+        raise ValueError('{}: checkpoint must be None or "8bit", got {!r}'.format(who, checkpoint))
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("{}: both biases or none".format(who))
+    if isinstance(w_gate, MX4Weights) or isinstance(w_up, MX4Weights):
+        if checkpoint is not None:
+            raise ValueError("{}: 4-bit weights have no backward pass to keep a checkpoint for".format(who))
+        return mx4_gated(x, w_gate, w_up, b_gate, b_up, activation)
+    code = dtype_code(x, who)
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[0] != x.shape[-1] or 0 in w_gate.shape:
+        raise ValueError("{}: kernels must both be [{}, units], got {} and {}".format(who, x.shape[-1] if x.dim() else "channels", tuple(w_gate.shape), tuple(w_up.shape)))
+    f = w_gate.shape[1]
+    params = [w_gate, w_up] + ([] if b_gate is None else [b_gate, b_up])
+    for p in params:
+        if p.device != x.device or p.dtype != w_gate.dtype or not (p.dtype == torch.float32 or (p.dtype == torch.bfloat16 and code == BF16)):
+            raise ValueError("{}: parameters must be float32 (or all bfloat16 under a bfloat16 input) on {}".format(who, x.device))
+    if b_gate is not None and (b_gate.shape != (f,) or b_up.shape != (f,)):
+        raise ValueError("{}: biases must be [{}], got {} and {}".format(who, f, tuple(b_gate.shape), tuple(b_up.shape)))
+    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+        return _GatedFn.apply(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation], checkpoint)
+    return _forward(x.detach(), _dense(w_gate.detach()), _dense(w_up.detach()), None if b_gate is None else b_gate.detach().contiguous(),
+                    None if b_up is None else b_up.detach().contiguous(), ACTIVATIONS[activation])
+
+
+class GatedFeedForward2D(object):
+    """The unit as a layer over NHWC tensors, in the manner of the pooling layers: parameters are made at the first call (he_normal
+    kernels as the bottlenecks', zero biases) from `seed`, or given with set_weights.  `checkpoint="8bit"` keeps the input in 8 bits
+    for the backward pass; `quantize()` returns the layer's answering form on 4-bit weights."""
+
+    def __init__(self, units, activation="swish", use_bias=True, checkpoint=None, seed=0, name=None, **kwargs):
+        if int(units) != units or units < 1:
+            raise ValueError("units must be a positive whole number, got {!r}".format(units))
+        if activation not in ACTIVATIONS:
+            raise ValueError("activation must be one of {}, got {!r}".format(sorted(ACTIVATIONS), activation))
+        if checkpoint not in (None, "8bit"):
+            raise ValueError('checkpoint must be None or "8bit", got {!r}'.format(checkpoint))
+        self.units, self.activation, self.use_bias, self.checkpoint, self.seed, self.name = int(units), activation, use_bias, checkpoint, seed, name
+        self.weights = None      # [gate kernel, up kernel(, gate bias, up bias)], float32
+
+    def build(self, input_shape, device="cuda"):
+        c = input_shape[-1]
+        g = torch.Generator().manual_seed(self.seed)
+        self.weights = [(torch.randn(c, self.units, generator=g) * (2.0 / c) ** 0.5).to(device).requires_grad_() for _ in range(2)]
+        if self.use_bias:
+            self.weights += [torch.zeros(self.units, device=device, requires_grad=True) for _ in range(2)]
+
+    def set_weights(self, weights, device="cuda"):
+        ws = [torch.as_tensor(w, dtype=torch.float32).detach().clone().to(device) for w in weights]
+        if len(ws) != (4 if self.use_bias else 2) or any(w.dim() != 2 or w.shape != ws[0].shape or w.shape[1] != self.units for w in ws[:2]) or \
+                any(b.shape != (self.units,) for b in ws[2:]):
+            raise ValueError("expected {} with {} units, got shapes {}".format("two kernels and two biases" if self.use_bias else "two kernels", self.units,
+                                                                               [tuple(w.shape) for w in ws]))
+        self.weights = [w.requires_grad_() for w in ws]
+
+    def get_weights(self):
+        return [w.detach().cpu().numpy() for w in self.weights or []]
+
+    def __call__(self, inputs, **kwargs):
+        require_gpu(inputs, type(self).__name__)
+        if self.weights is None:
+            self.build(inputs.shape, inputs.device)
+        return gated_feed_forward(inputs, *self.weights, activation=self.activation, checkpoint=self.checkpoint)
+
+    def quantize(self):
+        """A function of the input: the unit on 4-bit weights, made from the present ones."""
+        from .microscaled import quantize_mx4_weights
+        if self.weights is None:
+            raise ValueError("the layer has no weights yet")
+        kernels = [quantize_mx4_weights(w.detach()) for w in self.weights[:2]]
+        biases = [b.detach().clone() for b in self.weights[2:]]
+        return lambda x: gated_feed_forward(x, *kernels, *biases, activation=self.activation)
+
+    def compute_output_shape(self, input_shape):
+        return tuple(input_shape[:-1]) + (self.units,)
