@@ -141,49 +141,64 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_kernel(GateArgs a) 
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.c + S::W::kStepK - 1) / S::W::kStepK, acc);
 
-  const int r = lane & 31, hh = lane >> 5;
+  // a thread keeps four units for the whole epilogue
+  constexpr int kRounds = TileRows<SP, SQ>::kRows / (256 / (S::kHalf / 4));
+  const int f = f0 + (int)(threadIdx.x % (S::kHalf / 4)) * 4, n = a.f - f;
+  float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.bg) {
 #pragma unroll
-  for (int i = 0; i < SP / 2; ++i) {
+    for (int e = 0; e < 4; ++e) {
+      bg[e] = e < n ? param_at(a.bg, a.bf_params, f + e) : 0.f;
+      bu[e] = e < n ? param_at(a.bu, a.bf_params, f + e) : 0.f;
+    }
+  }
+  constexpr int kGroup = BWD ? 8 : 2, kGroups = BWD ? kRounds / kGroup : 1;
+  float dy[kGroups][BWD ? kGroup : 1][4];
+  tile_rows<SP, SQ, S::kHalf, kGroup>(
+      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (i / (SP / 2)) * S::kHalf + (s.wp * (SP / 2) + i % (SP / 2)) * 32; },
+      [&](int first, int per, auto q_of) {
+        if constexpr (BWD) {      // dy is on its way while the accumulators move
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int f = f0 + (s.wp * (SP / 2) + i) * 32 + 8 * k + 4 * hh;
-      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
-      if (a.bg) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bg[e] = f + e < a.f ? param_at(a.bg, a.bf_params, f + e) : 0.f;
-          bu[e] = f + e < a.f ? param_at(a.bu, a.bf_params, f + e) : 0.f;
+          for (int k = 0; k < kRounds; ++k) {
+            const int64_t m = m0 + q_of(first + k * per);
+            if (m < a.rows && n > 0) fetch4<T>(static_cast<const T*>(a.dy) + m * a.dy_ld + f, dy[k / kGroup][k % kGroup], n, a.vec_dy);
+          }
         }
-      }
-#pragma unroll
-      for (int j = 0; j < SQ; ++j) {
-        const int64_t m = m0 + (s.wq * SQ + j) * 32 + r;
-        if (m >= a.rows) continue;
+      },
+      [&](const float* row, int q, int col, int k) {
+        const int64_t m = m0 + q;
+        if (m >= a.rows || f >= (BWD ? a.fp : a.f)) return;
+        const f32x4 g = *reinterpret_cast<const f32x4*>(row + col), u = *reinterpret_cast<const f32x4*>(row + S::kHalf + col);
         float o[4];
         if constexpr (!BWD) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = gate_act<T>(a.act, acc[i][j][4 * k + e] + bg[e]) * (acc[i + SP / 2][j][4 * k + e] + bu[e]);
-          if (f < a.f) store4<T>(static_cast<T*>(a.out) + m * a.out_ld + f, o, a.f - f, a.vec_out);
+          for (int e = 0; e < 4; ++e) o[e] = gate_act<T>(a.act, g[e] + bg[e]) * (u[e] + bu[e]);
+          store4<T>(static_cast<T*>(a.out) + m * a.out_ld + f, o, n, a.vec_out);
         } else {
-          if (f >= a.fp) continue;
-          float dy[4], q[4];
-          fetch4<T>(static_cast<const T*>(a.dy) + m * a.dy_ld + f, dy, a.f - f, a.vec_dy);
+          float v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float u = acc[i + SP / 2][j][4 * k + e] + bu[e];
             float h, d;
-            gate_act_both<T>(a.act, acc[i][j][4 * k + e] + bg[e], h, d);
-            // padded units have dy = 0, but zero weights times an infinite x are no number: they are set, not multiplied
-            o[e] = f + e < a.f ? dy[e] * u * d : 0.f;
-            q[e] = f + e < a.f ? dy[e] * h : 0.f;
+            gate_act_both<T>(a.act, g[e] + bg[e], h, d);
+            // padded units are set, not multiplied: zero weights times an infinite x are no number
+            o[e] = e < n ? dy[0][k][e] * (u[e] + bu[e]) * d : 0.f;
+            v[e] = e < n ? dy[0][k][e] * h : 0.f;
           }
           T* const d = static_cast<T*>(a.out) + m * a.out_ld + f;
           Act<T>::gst4(d, f32x4{o[0], o[1], o[2], o[3]});
-          Act<T>::gst4(d + a.fp, f32x4{q[0], q[1], q[2], q[3]});
+          Act<T>::gst4(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
         }
-      }
-    }
-  }
+      },
+      [&] {
+        if constexpr (BWD) {
+#pragma unroll
+          for (int g = 0; g + 1 < kGroups; ++g)
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dy[g][k][e] = dy[g + 1][k][e];
+        }
+      });
 }
 
 // dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection
@@ -237,21 +252,17 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dx_kernel(GateDxArg
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, 2 * s.half, acc);
-  const int r = lane & 31, hh = lane >> 5;
-#pragma unroll
-  for (int j = 0; j < SQ; ++j) {
-    const int64_t m = m0 + (s.wq * SQ + j) * 32 + r;
-    if (m >= a.rows) continue;
-    T* const d = static_cast<T*>(a.dx) + m * a.dx_ld;
-#pragma unroll
-    for (int i = 0; i < SP; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = c0 + (s.wp * SP + i) * 32 + 8 * k + 4 * hh;
-        const float o[4] = {acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
-        if (c < a.c) store4<T>(d + c, o, a.c - c, a.vec_out);
-      }
-  }
+  tile_rows<SP, SQ, SP * 64, 4>(
+      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (s.wp * SP + i) * 32; }, [](int, int, auto) {},
+      [&](const float* row, int q, int col, int) {
+        const int64_t m = m0 + q;
+        const int c = c0 + col;
+        if (m >= a.rows || c >= a.c) return;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(row + col);
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        store4<T>(static_cast<T*>(a.dx) + m * a.dx_ld + c, o, a.c - c, a.vec_out);
+      },
+      [] {});
 }
 
 // part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]
@@ -299,20 +310,14 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dw_kernel(GateDwArg
   s.rx.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (s.rows + S::D::kStepK - 1) / S::D::kStepK, acc);
-  const int r = lane & 31, hh = lane >> 5;
-#pragma unroll
-  for (int j = 0; j < SQ; ++j) {
-    const int c = c0 + (s.wq * SQ + j) * 32 + r;
-    if (c >= a.c) continue;
-    float* const d = a.part + ((int64_t)strip * a.c + c) * (2 * (int64_t)a.fp);
-#pragma unroll
-    for (int i = 0; i < SP; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int p = p0 + (s.wp * SP + i) * 32 + 8 * k + 4 * hh;
-        if (p < 2 * a.fp) *reinterpret_cast<f32x4*>(d + p) = f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
-      }
-  }
+  tile_rows<SP, SQ, SP * 64, 4>(
+      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (s.wp * SP + i) * 32; }, [](int, int, auto) {},
+      [&](const float* row, int q, int col, int) {
+        const int c = c0 + q, p = p0 + col;
+        if (c < a.c && p < 2 * a.fp)
+          *reinterpret_cast<f32x4*>(a.part + ((int64_t)strip * a.c + c) * (2 * (int64_t)a.fp) + p) = *reinterpret_cast<const f32x4*>(row + col);
+      },
+      [] {});
 }
 
 // dW = sum of the strips' partial sums, in their order; four units a thread
@@ -572,12 +577,15 @@ static Staged stage_operands(const ssmi_gated_desc* d, const GatePlan& p, const 
   return s;
 }
 
+template <int SP, int SQ>
+static constexpr int tile_lds(int stages) { return stages > TileRows<SP, SQ>::kBytes ? stages : TileRows<SP, SQ>::kBytes; }
+
 template <typename T, int SP, int SQ, bool BWD>
 static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
   typedef GateSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), 2 * S::kStage, st, a);
+  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -590,7 +598,7 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), 2 * S::kStage, st, a);
+  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -599,7 +607,7 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   typedef DwSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
-  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), 2 * S::kStage, st, a);
+  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }

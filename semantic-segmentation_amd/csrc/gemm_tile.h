@@ -191,4 +191,52 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
   }
 }
 
+// The accumulators of a tile as rows in LDS, for an epilogue in memory order: q rows of 2 * 32 * SP float32 values, then `body(row, q,
+// col)` for every row and every fourth column under COLS, consecutive lanes on consecutive columns.  From the accumulator layout a
+// store touches 32 rows for 16 bytes each, and unrolling an epilogue over 256 registers overruns the instruction cache (the gated
+// unit's first form: 650 us for 65536 x 512 -> 2048, of which the products take 300).  Rows are padded by four values: the writes, one q
+// a lane, then step through the banks.  128 q rows go at a time (the large tile's 256 do not fit).
+// pos(i): first column of subtile i of this wave.
+template <int SP, int SQ>
+struct TileRows {
+  static constexpr int kWidth = SP * 64, kStride = kWidth + 4, kAtOnce = SQ > 2 ? 2 : SQ, kRows = 64 * kAtOnce;
+  static constexpr int kBytes = kRows * kStride * 4;
+};
+// Rounds go in groups of GROUP unrolled ones (`body`'s last argument counts inside a group, so it may index registers); early(first
+// row, rows per round, q_of) runs in front of a pass's LDS writes, next() behind every group.
+template <int SP, int SQ, int COLS, int GROUP, typename Pos, typename Early, typename Body, typename Next>
+__device__ __forceinline__ void tile_rows(const f32x16 (&acc)[SP][SQ], float* lds, int wq, Pos pos, Early early, Body body, Next next) {
+  typedef TileRows<SP, SQ> R;
+  constexpr int kLanes = COLS / 4, kPerRound = 256 / kLanes, kRounds = R::kRows / kPerRound;
+  const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5;
+  const int col = (threadIdx.x % kLanes) * 4, first = threadIdx.x / kLanes;
+#pragma unroll
+  for (int pass = 0; pass < SQ / R::kAtOnce; ++pass) {
+    auto q_of = [&](int row) { return (row / (32 * R::kAtOnce)) * (32 * SQ) + pass * (32 * R::kAtOnce) + row % (32 * R::kAtOnce); };
+    early(first, kPerRound, q_of);
+    if (pass) __syncthreads();
+#pragma unroll
+    for (int jj = 0; jj < R::kAtOnce; ++jj)
+#pragma unroll
+      for (int i = 0; i < SP; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f32x16& a = acc[i][pass * R::kAtOnce + jj];
+          *reinterpret_cast<f32x4*>(lds + (wq * (32 * R::kAtOnce) + jj * 32 + r) * R::kStride + pos(i) + 8 * k + 4 * hh) =
+              f32x4{a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]};
+        }
+    __syncthreads();
+    static_assert(kRounds % GROUP == 0, "whole groups");
+#pragma unroll 1
+    for (int n = 0; n < kRounds; n += GROUP) {
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const int row = first + (n + i) * kPerRound;
+        body(lds + row * R::kStride, q_of(row), col, i);
+      }
+      next();
+    }
+  }
+}
+
 }  // namespace ssmi
