@@ -25,24 +25,24 @@ template <typename T>
 __device__ __forceinline__ float gate_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-v));      // exp = inf gives 0
 }
-template <typename T>
-__device__ __forceinline__ float gate_act(int act, float g) {
-  if (act == kSwish) return g * gate_sigmoid<T>(g);
-  if (act == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678f));
-  if (act == kRelu) return fmaxf(g, 0.f);
+template <typename T, int ACT>
+__device__ __forceinline__ float gate_act(float g) {
+  if constexpr (ACT == kSwish) return g * gate_sigmoid<T>(g);
+  if constexpr (ACT == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678f));
+  if constexpr (ACT == kRelu) return fmaxf(g, 0.f);
   return gate_sigmoid<T>(g);
 }
-template <typename T>
-__device__ __forceinline__ void gate_act_both(int act, float g, float& a, float& d) {
-  if (act == kSwish) {
+template <typename T, int ACT>
+__device__ __forceinline__ void gate_act_both(float g, float& a, float& d) {
+  if constexpr (ACT == kSwish) {
     const float s = gate_sigmoid<T>(g);
     a = g * s;
     d = s * (1.f + g * (1.f - s));
-  } else if (act == kGelu) {
+  } else if constexpr (ACT == kGelu) {
     const float c = 0.5f * (1.f + erff(g * 0.70710678f));
     a = g * c;
     d = c + g * 0.39894228f * gate_exp<T>(-0.5f * g * g);
-  } else if (act == kRelu) {
+  } else if constexpr (ACT == kRelu) {
     a = fmaxf(g, 0.f);
     d = g > 0.f ? 1.f : 0.f;
   } else {
@@ -51,19 +51,37 @@ __device__ __forceinline__ void gate_act_both(int act, float g, float& a, float&
   }
 }
 
+// runs body(integral constant) for the activation: one branch around an epilogue, none inside it
+template <int V> struct ActIs { static constexpr int value = V; };
+template <typename Body>
+__device__ __forceinline__ void with_act(int act, Body body) {
+  if (act == kSwish) body(ActIs<kSwish>{});
+  else if (act == kGelu) body(ActIs<kGelu>{});
+  else if (act == kRelu) body(ActIs<kRelu>{});
+  else body(ActIs<kSigmoid>{});
+}
+
 __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
   return bf ? (float)static_cast<const bf16*>(p)[i] : static_cast<const float*>(p)[i];
 }
 
 // Which (p, q) tile a workgroup takes.  Consecutive workgroups of an XCD walk kGroupQ row tiles under one column tile, then the
-// next column tile: 32 CUs of an XCD share about eight row tiles and four column tiles through their L2.
-static constexpr int kGroupQ = 8;
+// next column tile: the workgroups of an XCD that run together share a few row tiles and column tiles through its L2
+// (1, 2, 4, 8, 16 measured within 3 % of each other).
+static constexpr int kGroupQ = 4;
 struct TileAt { int p, q; };
 __device__ __forceinline__ TileAt tile_at(unsigned v, unsigned np, unsigned nq) {
   const unsigned per = kGroupQ * np, grp = v / per, in = v - grp * per;
   const unsigned gq = min((unsigned)kGroupQ, nq - grp * kGroupQ);
-  return {(int)(in / gq), (int)(grp * kGroupQ + in % gq)};
+  // divisions run on the vector unit: back to scalars, the tile's addresses hang on them
+  return {(int)__builtin_amdgcn_readfirstlane(in / gq), (int)__builtin_amdgcn_readfirstlane(grp * kGroupQ + in % gq)};
 }
+
+// Stages and K step of a tile shape, and how many of its workgroups a CU holds (registers and LDS)
+template <int SP, int SQ>
+struct TileShape {
+  static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kPerCu = SP * SQ == 16 ? 1 : 2;
+};
 
 struct GateArgs {
   const void *x, *wg, *wu;      // x [rows][x_ld], W [c][w_ld], activation type
@@ -77,11 +95,12 @@ struct GateArgs {
 };
 
 template <typename T, int SP, int SQ>
-struct GateSides {
+struct GateSides : TileShape<SP, SQ> {
+  using TileShape<SP, SQ>::kStep;
   static constexpr int kHalf = SP * 32;      // units of a tile
-  typedef Operand<T, kHalf, true> W;
-  typedef Operand<T, SQ * 64, false> X;
-  static constexpr int kStage = 2 * W::kBytes + X::kBytes;
+  typedef Operand<T, kHalf, true, kStep> W;
+  typedef Operand<T, SQ * 64, false, kStep> X;
+  static constexpr int kStage = 2 * W::kBytes + X::kBytes, kLoads = 2 * W::kLoads + X::kLoads;
   W wg, wu;
   X x;
   typename W::Reader rw;
@@ -122,7 +141,7 @@ __device__ __forceinline__ void fetch4(const T* p, float (&v)[4], int n, bool ve
 }
 
 template <typename T, int SP, int SQ, bool BWD>
-__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_kernel(GateArgs a) {
+__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef GateSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -142,8 +161,8 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_kernel(GateArgs a) 
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.c + S::W::kStepK - 1) / S::W::kStepK, acc);
 
   // a thread keeps four units for the whole epilogue
-  constexpr int kRounds = TileRows<SP, SQ>::kRows / (256 / (S::kHalf / 4));
-  const int f = f0 + (int)(threadIdx.x % (S::kHalf / 4)) * 4, n = a.f - f;
+  typedef TileRows<SP, SQ, S::kHalf> R;
+  const int col = R::col(), f = f0 + col, n = a.f - f;
   float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
   if (a.bg) {
 #pragma unroll
@@ -152,53 +171,79 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_kernel(GateArgs a) 
       bu[e] = e < n ? param_at(a.bu, a.bf_params, f + e) : 0.f;
     }
   }
-  constexpr int kGroup = BWD ? 8 : 2, kGroups = BWD ? kRounds / kGroup : 1;
-  float dy[kGroups][BWD ? kGroup : 1][4];
-  tile_rows<SP, SQ, S::kHalf, kGroup>(
-      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (i / (SP / 2)) * S::kHalf + (s.wp * (SP / 2) + i % (SP / 2)) * 32; },
-      [&](int first, int per, auto q_of) {
-        if constexpr (BWD) {      // dy is on its way while the accumulators move
+  const int wp = s.wp;
+  auto pos = [&](int i) __attribute__((always_inline)) { return (i / (SP / 2)) * S::kHalf + (wp * (SP / 2) + i % (SP / 2)) * 32; };
+  const bool whole = m0 + SQ * 64 <= a.rows && f0 + S::kHalf <= a.f && a.vec_out && (!BWD || a.vec_dy);      // uniform
+  // the lane's place in a tile of `out` / dy; rounds add whole rows
+  T* const out = static_cast<T*>(a.out) + m0 * a.out_ld + f0;
+  const T* const dyt = static_cast<const T*>(a.dy) + (BWD ? m0 * a.dy_ld + f0 : 0);
+  const unsigned o_lane = (unsigned)R::first() * (unsigned)a.out_ld + (unsigned)col, d_lane = (unsigned)R::first() * (unsigned)a.dy_ld + (unsigned)col;
+  with_act(a.act, [&](auto which) __attribute__((always_inline)) {
+    constexpr int kAct = decltype(which)::value;
+    auto forward = [&](const float* row, float (&o)[4]) __attribute__((always_inline)) {
+      const f32x4 g = *reinterpret_cast<const f32x4*>(row), u = *reinterpret_cast<const f32x4*>(row + S::kHalf);
 #pragma unroll
-          for (int k = 0; k < kRounds; ++k) {
-            const int64_t m = m0 + q_of(first + k * per);
-            if (m < a.rows && n > 0) fetch4<T>(static_cast<const T*>(a.dy) + m * a.dy_ld + f, dy[k / kGroup][k % kGroup], n, a.vec_dy);
-          }
-        }
-      },
-      [&](const float* row, int q, int col, int k) {
-        const int64_t m = m0 + q;
-        if (m >= a.rows || f >= (BWD ? a.fp : a.f)) return;
-        const f32x4 g = *reinterpret_cast<const f32x4*>(row + col), u = *reinterpret_cast<const f32x4*>(row + S::kHalf + col);
-        float o[4];
-        if constexpr (!BWD) {
+      for (int e = 0; e < 4; ++e) o[e] = gate_act<T, kAct>(g[e] + bg[e]) * (u[e] + bu[e]);
+    };
+    auto backward = [&](const float* row, const float (&dy)[4], float (&o)[4], float (&v)[4]) __attribute__((always_inline)) {
+      const f32x4 g = *reinterpret_cast<const f32x4*>(row), u = *reinterpret_cast<const f32x4*>(row + S::kHalf);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = gate_act<T>(a.act, g[e] + bg[e]) * (u[e] + bu[e]);
-          store4<T>(static_cast<T*>(a.out) + m * a.out_ld + f, o, n, a.vec_out);
-        } else {
-          float v[4];
+      for (int e = 0; e < 4; ++e) {
+        float h, d;
+        gate_act_both<T, kAct>(g[e] + bg[e], h, d);
+        o[e] = dy[e] * (u[e] + bu[e]) * d;
+        v[e] = dy[e] * h;
+      }
+    };
+    if (whole) {
+      typename Act<T>::raw4 dy[BWD ? R::kRounds : 1];
+      R::template run<R::kRounds>(
+          acc, reinterpret_cast<float*>(smem), s.wq, pos,
+          [&](int pass) __attribute__((always_inline)) {
+            if constexpr (BWD) {      // dy is on its way while the accumulators move
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float h, d;
-            gate_act_both<T>(a.act, g[e] + bg[e], h, d);
-            // padded units are set, not multiplied: zero weights times an infinite x are no number
-            o[e] = e < n ? dy[0][k][e] * (u[e] + bu[e]) * d : 0.f;
-            v[e] = e < n ? dy[0][k][e] * h : 0.f;
-          }
-          T* const d = static_cast<T*>(a.out) + m * a.out_ld + f;
-          Act<T>::gst4(d, f32x4{o[0], o[1], o[2], o[3]});
-          Act<T>::gst4(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
-        }
-      },
-      [&] {
-        if constexpr (BWD) {
+              for (int i = 0; i < R::kRounds; ++i) dy[i] = *reinterpret_cast<const typename Act<T>::raw4*>(dyt + R::q_of(pass, i) * a.dy_ld + d_lane);
+            }
+          },
+          [&](const float* row, int qc, int i) __attribute__((always_inline)) {
+            float o[4], v[4];
+            T* const d = out + qc * a.out_ld + o_lane;
+            if constexpr (!BWD) {
+              forward(row, o);
+            } else {
+              const f32x4 y = Act<T>::up4(dy[i]);
+              const float y4[4] = {y[0], y[1], y[2], y[3]};
+              backward(row, y4, o, v);
+              put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
+            }
+            put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
+          });
+    } else {
+      R::template run<1>(
+          acc, reinterpret_cast<float*>(smem), s.wq, pos, [](int) {},
+          [&](const float* row, int qc, int) __attribute__((always_inline)) {
+            const int64_t m = m0 + R::first() + qc;
+            if (m >= a.rows || f >= (BWD ? a.fp : a.f)) return;
+            float o[4], v[4];
+            T* const d = static_cast<T*>(a.out) + m * a.out_ld + f;
+            if constexpr (!BWD) {
+              forward(row, o);
+              store4<T>(d, o, n, a.vec_out);
+            } else {
+              float dy[4];
+              fetch4<T>(static_cast<const T*>(a.dy) + m * a.dy_ld + f, dy, n, a.vec_dy);
+              backward(row, dy, o, v);
 #pragma unroll
-          for (int g = 0; g + 1 < kGroups; ++g)
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) dy[g][k][e] = dy[g + 1][k][e];
-        }
-      });
+              for (int e = 0; e < 4; ++e) {      // padded units are set, not multiplied: zero weights times an infinite x are no number
+                o[e] = e < n ? o[e] : 0.f;
+                v[e] = e < n ? v[e] : 0.f;
+              }
+              put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
+              put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
+            }
+          });
+    }
+  });
 }
 
 // dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection
@@ -210,10 +255,11 @@ struct GateDxArgs {
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
-struct DxSides {
-  typedef Operand<T, SP * 64, false> W;
-  typedef Operand<T, SQ * 64, false> D;
-  static constexpr int kStage = W::kBytes + D::kBytes;
+struct DxSides : TileShape<SP, SQ> {
+  using TileShape<SP, SQ>::kStep;
+  typedef Operand<T, SP * 64, false, kStep> W;
+  typedef Operand<T, SQ * 64, false, kStep> D;
+  static constexpr int kStage = W::kBytes + D::kBytes, kLoads = W::kLoads + D::kLoads;
   W wg;
   D d;
   __amdgpu_buffer_rsrc_t wu;
@@ -233,7 +279,7 @@ struct DxSides {
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rd.get(s + W::kBytes, wq * SQ + j, ks); }
 };
 template <typename T, int SP, int SQ>
-__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dx_kernel(GateDxArgs a) {
+__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dx_kernel(GateDxArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef DxSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -252,17 +298,24 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dx_kernel(GateDxArg
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, 2 * s.half, acc);
-  tile_rows<SP, SQ, SP * 64, 4>(
-      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (s.wp * SP + i) * 32; }, [](int, int, auto) {},
-      [&](const float* row, int q, int col, int) {
-        const int64_t m = m0 + q;
-        const int c = c0 + col;
-        if (m >= a.rows || c >= a.c) return;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(row + col);
-        const float o[4] = {v[0], v[1], v[2], v[3]};
-        store4<T>(static_cast<T*>(a.dx) + m * a.dx_ld + c, o, a.c - c, a.vec_out);
-      },
-      [] {});
+  typedef TileRows<SP, SQ, SP * 64> R;
+  const int wp = s.wp, c = c0 + R::col();
+  auto pos = [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; };
+  if (m0 + SQ * 64 <= a.rows && c0 + SP * 64 <= a.c && a.vec_out) {
+    T* const dx = static_cast<T*>(a.dx) + m0 * a.dx_ld + c0;
+    const unsigned lane_at = (unsigned)R::first() * (unsigned)a.dx_ld + (unsigned)R::col();
+    R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), s.wq, pos, [](int) {}, [&](const float* row, int qc, int) __attribute__((always_inline)) {
+      put4<T>(dx + qc * a.dx_ld + lane_at, *reinterpret_cast<const f32x4*>(row));
+    });
+  } else {
+    R::template run<1>(acc, reinterpret_cast<float*>(smem), s.wq, pos, [](int) {}, [&](const float* row, int qc, int) __attribute__((always_inline)) {
+      const int64_t m = m0 + R::first() + qc;
+      if (m >= a.rows || c >= a.c) return;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(row);
+      const float o[4] = {v[0], v[1], v[2], v[3]};
+      store4<T>(static_cast<T*>(a.dx) + m * a.dx_ld + c, o, a.c - c, a.vec_out);
+    });
+  }
 }
 
 // part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]
@@ -274,10 +327,11 @@ struct GateDwArgs {
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
-struct DwSides {
-  typedef Operand<T, SP * 64, true> D;
-  typedef Operand<T, SQ * 64, true> X;
-  static constexpr int kStage = D::kBytes + X::kBytes;
+struct DwSides : TileShape<SP, SQ> {
+  using TileShape<SP, SQ>::kStep;
+  typedef Operand<T, SP * 64, true, kStep> D;
+  typedef Operand<T, SQ * 64, true, kStep> X;
+  static constexpr int kStage = D::kBytes + X::kBytes, kLoads = D::kLoads + X::kLoads;
   D d;
   X x;
   typename D::Reader rd;
@@ -292,11 +346,11 @@ struct DwSides {
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + D::kBytes, wq * SQ + j, ks); }
 };
 template <typename T, int SP, int SQ>
-__global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dw_kernel(GateDwArgs a) {
+__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dw_kernel(GateDwArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef DwSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const unsigned v = spread_blocks(blockIdx.x, gridDim.x), tiles = a.np * a.nq, strip = v / tiles;
+  const unsigned v = spread_blocks(blockIdx.x, gridDim.x), tiles = a.np * a.nq, strip = __builtin_amdgcn_readfirstlane(v / tiles);
   const TileAt at = tile_at(v - strip * tiles, a.np, a.nq);
   const int64_t m0 = (int64_t)strip * a.strip_rows;
   const int c0 = at.q * (SQ * 64), p0 = at.p * (SP * 64);
@@ -310,14 +364,13 @@ __global__ __launch_bounds__(256, SP == 4 ? 1 : 2) void gate_dw_kernel(GateDwArg
   s.rx.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (s.rows + S::D::kStepK - 1) / S::D::kStepK, acc);
-  tile_rows<SP, SQ, SP * 64, 4>(
-      acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) { return (s.wp * SP + i) * 32; }, [](int, int, auto) {},
-      [&](const float* row, int q, int col, int) {
-        const int c = c0 + q, p = p0 + col;
-        if (c < a.c && p < 2 * a.fp)
-          *reinterpret_cast<f32x4*>(a.part + ((int64_t)strip * a.c + c) * (2 * (int64_t)a.fp) + p) = *reinterpret_cast<const f32x4*>(row + col);
-      },
-      [] {});
+  typedef TileRows<SP, SQ, SP * 64> R;
+  const int wp = s.wp, p = p0 + R::col();
+  float* const part = a.part + ((int64_t)strip * a.c + c0 + R::first()) * (2 * (int64_t)a.fp) + p;
+  R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; }, [](int) {},
+                              [&](const float* row, int qc, int) __attribute__((always_inline)) {
+                                if (c0 + R::first() + qc < a.c && p < 2 * a.fp) *reinterpret_cast<f32x4*>(part + qc * (2 * (int64_t)a.fp)) = *reinterpret_cast<const f32x4*>(row);
+                              });
 }
 
 // dW = sum of the strips' partial sums, in their order; four units a thread
@@ -460,7 +513,8 @@ __global__ __launch_bounds__(256) void gate_rows_kernel(GateArgs a) {
       g += param_at(a.bg, a.bf_params, ff);
       u += param_at(a.bu, a.bf_params, ff);
     }
-    Act<T>::gst(static_cast<T*>(a.out) + (m0 + m) * a.out_ld + ff, gate_act<T>(a.act, g) * u);
+    with_act(a.act, [&](auto which) { g = gate_act<T, decltype(which)::value>(g); });
+    Act<T>::gst(static_cast<T*>(a.out) + (m0 + m) * a.out_ld + ff, g * u);
   }
 }
 
@@ -578,27 +632,27 @@ static Staged stage_operands(const ssmi_gated_desc* d, const GatePlan& p, const 
 }
 
 template <int SP, int SQ>
-static constexpr int tile_lds(int stages) { return stages > TileRows<SP, SQ>::kBytes ? stages : TileRows<SP, SQ>::kBytes; }
+static constexpr int tile_lds(int stages) { return stages > TileRows<SP, SQ, 64>::kBytes ? stages : TileRows<SP, SQ, 64>::kBytes; }
 
 template <typename T, int SP, int SQ, bool BWD>
 static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
   typedef GateSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
 template <typename T, bool BWD>
 static ssmi_status launch_gate(const GateArgs& a, hipStream_t st) {
-  return wants_big(a.rows, 2 * (int64_t)a.f) ? launch_gate_as<T, 4, 4, BWD>(a, st) : launch_gate_as<T, 2, 2, BWD>(a, st);
+  return wants_big(a.rows, 2 * (int64_t)a.f) ? launch_gate_as<T, 2, 4, BWD>(a, st) : launch_gate_as<T, 2, 2, BWD>(a, st);
 }
 template <typename T, int SP, int SQ>
 static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -607,7 +661,7 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   typedef DwSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
-  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<SP, SQ>(2 * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -663,6 +717,7 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.bg = bg; a.bu = bu; a.dy = dy; a.out = dgu;
   a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = 2 * (int64_t)p.fp; a.dy_ld = d->y_ld;
   a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf;
+  a.vec_out = 1;
   a.vec_dy = d->y_ld % 4 == 0 && aligned(dy, 4 * p.es);
   ssmi_status r = launch_gate<T, true>(a, st);
   if (r != SSMI_OK) return r;
@@ -676,7 +731,7 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   if (dwg || dwu) {
     GateDwArgs b = {};
     b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp;
-    r = p.big_dw ? launch_dw_as<T, 4, 4>(b, p.strips, st) : launch_dw_as<T, 2, 2>(b, p.strips, st);
+    r = p.big_dw ? launch_dw_as<T, 2, 4>(b, p.strips, st) : launch_dw_as<T, 2, 2>(b, p.strips, st);
     if (r != SSMI_OK) return r;
     hipLaunchKernelGGL(gate_dw_reduce, dim3((unsigned)ceil_div64((int64_t)d->c * (p.fp / 2), 256)), dim3(256), 0, st, part, p.strips, (int64_t)d->c, d->f, p.fp, dwg, dwu, bf);
     SSMI_LAUNCH_CHECK();

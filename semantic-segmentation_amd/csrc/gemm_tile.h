@@ -5,14 +5,15 @@
 // contiguous axis: the accumulator layout of the 32x32 instructions gives a lane one q and runs of four consecutive p, i.e. vector
 // stores and epilogues that see a pixel's neighbouring channels.
 // Either operand comes in one of two memory forms:
-//   rows:  [index][k], k contiguous             - staged as 128-byte rows, read back with ds_read_b128
+//   rows:  [index][k], k contiguous             - staged as rows of STEP bytes, read back with ds_read_b128
 //   cols:  [k][index], index contiguous         - staged as k rows, read back transposed (ds_read_tr16_b64 for bfloat16, single words
 //                                                 for float32), so Keras kernels [in][out] and weight gradients need no transposed copy
-// A K step is 128 bytes of a row: 64 bfloat16 or 32 float32 values.  Four waves split the tile 2 x 2; a wave owns SP x SQ
+// A K step is STEP = 128 or 64 bytes of a row: 64 or 32 bfloat16, half as many float32 values.  Four waves split the tile 2 x 2; a wave owns SP x SQ
 // accumulators of 32 x 32.
 // Staging: global -> LDS directly, 16 bytes a lane; the LDS image is linear in the lane order, so the swizzle against bank conflicts
 // is applied to the source: slot s of a row holds piece s ^ f(row), f chosen so that one read of a wave spreads over all banks.
-// Two stages: the loads of step t + 1 are issued behind the one barrier of step t and have its whole arithmetic to arrive.
+// kStages stages: a step's one barrier sits in front of its last fragments' arithmetic; behind it the stage is free for the loads of
+// step t + kStages, which then have the arithmetic of kStages - 1 steps to arrive.
 // Lanes that must see zeros (past the last row, past K) pass an out-of-range offset; the buffer check returns zeros.
 // Everything is addressed from a per-tile 64-bit base, so tensors may be larger than 2 GiB; a tile's own extent may not.
 #pragma once
@@ -24,8 +25,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char* lds_bytes;
 
-static constexpr int kStepBytes = 128;
-
 __device__ __forceinline__ unsigned spread_blocks(unsigned b, unsigned n) {      // workgroups of one XCD take consecutive tiles (a bijection of [0, n))
   const unsigned q = n >> 3, r = n & 7u, x = b & 7u;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);
@@ -33,20 +32,23 @@ __device__ __forceinline__ unsigned spread_blocks(unsigned b, unsigned n) {     
 
 // 64 lanes x 16 bytes from buffer offsets to LDS bytes [at, at + 1024), `at` uniform.  In assembly because the compiler, which cannot
 // tell the two stages apart, would wait for every such load in front of the next LDS read; nothing is returned in registers, and the
-// tile loop waits for them itself (stage_wait) in front of the barrier that publishes a stage.
+// tile loop waits for them itself (stage_wait, in order) in front of the barrier that publishes a stage.
 __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, unsigned at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
-__device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void stage_wait() {      // until at most LEFT loads are on their way
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
 
-// One operand of one tile.  N: indices of the tile (p or q), COLS: memory form.
-template <typename T, int N, bool COLS>
+// One operand of one tile.  N: indices of the tile (p or q), COLS: memory form, STEP: bytes of a K step.
+template <typename T, int N, bool COLS, int STEP>
 struct Operand {
   static constexpr int kElems = 16 / (int)sizeof(T);                 // values per 16-byte piece
-  static constexpr int kStepK = kStepBytes / (int)sizeof(T);
-  static constexpr int kBytes = N * kStepBytes;                      // LDS bytes of one stage
+  static constexpr int kStepK = STEP / (int)sizeof(T);
+  static constexpr int kBytes = N * STEP;                      // LDS bytes of one stage
   static constexpr int kLoads = kBytes / 4096;                       // per lane and step
-  static constexpr int kRowBytes = COLS ? N * (int)sizeof(T) : kStepBytes;
+  static constexpr int kRowBytes = COLS ? N * (int)sizeof(T) : STEP;
   static constexpr int kRowsPerLoad = 4096 / kRowBytes;              // LDS rows that the workgroup stages with one load per lane
   static_assert(kBytes % 4096 == 0, "whole loads");
 
@@ -56,7 +58,7 @@ struct Operand {
   unsigned step_bytes;           // buffer offset from one K step to the next
 
   static __device__ __forceinline__ int swizzle(int row) {
-    if constexpr (!COLS) return row & 7;
+    if constexpr (!COLS) return STEP == 128 ? row & 7 : (row >> 2) & 3;
     if constexpr (sizeof(T) == 2) return kRowBytes >= 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
     return ((row >> 2) & 1) << 3;
   }
@@ -65,8 +67,8 @@ struct Operand {
   __device__ __forceinline__ void init(const T* base, int64_t ld, int count) {
     rsrc = make_rsrc(base, 0x7FFFFFFFu);
     const int tid = threadIdx.x;
-    constexpr int kPieces = kRowBytes / 16;
-    const int row = tid / kPieces, slot = tid % kPieces;
+    constexpr int kRowPieces = kRowBytes / 16;
+    const int row = tid / kRowPieces, slot = tid % kRowPieces;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int rj = row + j * kRowsPerLoad;
@@ -79,17 +81,19 @@ struct Operand {
         if (j == 0) k_in = piece * kElems;      // the same for every load: rows advance by multiples of eight
       }
     }
-    step_bytes = COLS ? (unsigned)(ld * (kStepK * (int64_t)sizeof(T))) : (unsigned)kStepBytes;
+    step_bytes = COLS ? (unsigned)(ld * (kStepK * (int64_t)sizeof(T))) : (unsigned)STEP;
   }
 
   // requests K step t into the stage at `lds`; left: valid k from this step's first on; skip: bytes in front of step 0
   __device__ __forceinline__ void request(lds_bytes lds, int t, int left, unsigned skip = 0) const {
     const unsigned soff = (unsigned)t * step_bytes + skip;
     const unsigned dst = (unsigned)(uintptr_t)lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    if (left >= kStepK) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int k = COLS ? k_in + j * kRowsPerLoad : k_in;
-      stage16(rsrc, k < left ? voff[j] : kOOB, soff, dst + j * 4096);
+      for (int j = 0; j < kLoads; ++j) stage16(rsrc, voff[j], soff, dst + j * 4096);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) stage16(rsrc, (COLS ? k_in + j * kRowsPerLoad : k_in) < left ? voff[j] : kOOB, soff, dst + j * 4096);
     }
   }
 
@@ -99,7 +103,7 @@ struct Operand {
     __device__ __forceinline__ void init(int lane) {
       const int r = lane & 31, hh = lane >> 5;
       if constexpr (!COLS) {
-        at = (unsigned)(r * kStepBytes + ((hh ^ (r & 7)) << 4));
+        at = (unsigned)(r * STEP + ((hh ^ swizzle(r)) << 4));
       } else if constexpr (sizeof(T) == 2) {
         const int sq = (lane >> 2) & 3, sp = lane & 3, gh = (lane >> 4) & 1;
         const int row = 8 * hh + sq;
@@ -110,7 +114,7 @@ struct Operand {
     }
     __device__ __forceinline__ u32x4 get(lds_bytes stage, int s, int ks) const {
       if constexpr (!COLS) {
-        return *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(stage + s * 32 * kStepBytes + (at ^ (unsigned)(ks << 5)));
+        return *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(stage + s * 32 * STEP + (at ^ (unsigned)(ks << 5)));
       } else if constexpr (sizeof(T) == 2) {
         // subtiles lie 64 bytes apart inside the swizzled 256 (128) bytes
         constexpr int kIn = kRowBytes >= 256 ? 4 : 2;
@@ -169,73 +173,85 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
 #pragma unroll
       for (int j = 0; j < SQ; ++j) acc[i][j] = mfma_step<T>(p[buf][i], q[buf][j], acc[i][j]);
   };
-  sides.request(lds, 0);
-  stage_wait();
+  constexpr int kStages = Sides::kStages, kPieces = Sides::kStep / 32, kAhead = (kStages - 2) * Sides::kLoads;
+  for (int t = 0; t < kStages && t < steps; ++t) sides.request(lds + t * kStage, t);
+  if (steps >= kStages) stage_wait<(kStages - 1) * Sides::kLoads>();
+  else stage_wait<0>();
   __syncthreads();
-  if (steps > 1) sides.request(lds + kStage, 1);
   read(0, lds, 0);
+  int at = 0;
   for (int t = 0; t < steps; ++t) {
-    lds_bytes cur = lds + (t & 1) * kStage, nxt = lds + ((t + 1) & 1) * kStage;
-    read(1, cur, 1);
-    multiply(0);
-    read(0, cur, 2);
-    multiply(1);
-    read(1, cur, 3);
-    multiply(0);
-    stage_wait();
-    __syncthreads();      // step t + 1 is there, and nobody reads step t any more
+    lds_bytes cur = lds + at * kStage;
+    at = at + 1 == kStages ? 0 : at + 1;
+    lds_bytes nxt = lds + at * kStage;
+#pragma unroll
+    for (int ks = 0; ks + 1 < kPieces; ++ks) {
+      read((ks + 1) & 1, cur, ks + 1);
+      multiply(ks & 1);
+    }
+    if (t + kStages <= steps) stage_wait<kAhead>();      // all of steps t + 1 .. t + kStages - 1 were requested: the first is there
+    else stage_wait<0>();
+    __syncthreads();      // step t + 1 is there for everyone, and nobody reads step t any more
     __builtin_amdgcn_sched_barrier(0);
-    if (t + 2 < steps) sides.request(cur, t + 2);
+    if (t + kStages < steps) sides.request(cur, t + kStages);
     if (t + 1 < steps) read(0, nxt, 0);
     multiply(1);
   }
 }
 
-// The accumulators of a tile as rows in LDS, for an epilogue in memory order: q rows of 2 * 32 * SP float32 values, then `body(row, q,
-// col)` for every row and every fourth column under COLS, consecutive lanes on consecutive columns.  From the accumulator layout a
-// store touches 32 rows for 16 bytes each, and unrolling an epilogue over 256 registers overruns the instruction cache (the gated
-// unit's first form: 650 us for 65536 x 512 -> 2048, of which the products take 300).  Rows are padded by four values: the writes, one q
-// a lane, then step through the banks.  128 q rows go at a time (the large tile's 256 do not fit).
-// pos(i): first column of subtile i of this wave.
-template <int SP, int SQ>
+// The accumulators of a tile as rows in LDS, for an epilogue in memory order: q rows of 2 * 32 * SP float32 values; consecutive lanes
+// take consecutive columns, four each, out of COLS.  From the accumulator layout a store would touch 32 rows for 16 bytes each.  Rows
+// are padded by four values: the writes, one q a lane, then step through the banks.  64 * kAtOnce q rows go at a time.
+//   pos(i)                     first column of subtile i of this wave
+//   early(pass)                in front of a pass's LDS writes
+//   round(row, qc, i)          the lane's row of LDS values and its q: first() + qc.  UNROLL = kRounds makes qc and i constants, so that
+//                              an epilogue without branches keeps many rounds in flight and addresses its rows with scalars.
+template <int SP, int SQ, int COLS>
 struct TileRows {
-  static constexpr int kWidth = SP * 64, kStride = kWidth + 4, kAtOnce = SQ > 2 ? 2 : SQ, kRows = 64 * kAtOnce;
+  static constexpr int kWidth = SP * 64, kStride = kWidth + 4, kAtOnce = SQ > 2 ? 2 : SQ, kRows = 64 * kAtOnce, kPasses = SQ / kAtOnce;
   static constexpr int kBytes = kRows * kStride * 4;
-};
-// Rounds go in groups of GROUP unrolled ones (`body`'s last argument counts inside a group, so it may index registers); early(first
-// row, rows per round, q_of) runs in front of a pass's LDS writes, next() behind every group.
-template <int SP, int SQ, int COLS, int GROUP, typename Pos, typename Early, typename Body, typename Next>
-__device__ __forceinline__ void tile_rows(const f32x16 (&acc)[SP][SQ], float* lds, int wq, Pos pos, Early early, Body body, Next next) {
-  typedef TileRows<SP, SQ> R;
-  constexpr int kLanes = COLS / 4, kPerRound = 256 / kLanes, kRounds = R::kRows / kPerRound;
-  const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5;
-  const int col = (threadIdx.x % kLanes) * 4, first = threadIdx.x / kLanes;
+  static constexpr int kLanes = COLS / 4, kPerRound = 256 / kLanes, kRounds = kRows / kPerRound, kHalf = 32 * kAtOnce;
+  static_assert(kHalf % kPerRound == 0 && COLS <= kWidth, "rounds stay inside a wave's rows");
+  static __device__ __forceinline__ int first() { return (int)threadIdx.x / kLanes; }
+  static __device__ __forceinline__ int col() { return (int)(threadIdx.x % kLanes) * 4; }
+  static __device__ __forceinline__ constexpr int q_of(int pass, int i) {
+    return (i * kPerRound / kHalf) * (32 * SQ) + pass * kHalf + i * kPerRound % kHalf;
+  }
+  template <int UNROLL, typename Pos, typename Early, typename Round>
+  static __device__ __forceinline__ void run(const f32x16 (&acc)[SP][SQ], float* lds, int wq, Pos pos, Early early, Round round) {
+    const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5;
+    const float* const mine = lds + first() * kStride + col();
 #pragma unroll
-  for (int pass = 0; pass < SQ / R::kAtOnce; ++pass) {
-    auto q_of = [&](int row) { return (row / (32 * R::kAtOnce)) * (32 * SQ) + pass * (32 * R::kAtOnce) + row % (32 * R::kAtOnce); };
-    early(first, kPerRound, q_of);
-    if (pass) __syncthreads();
+    for (int pass = 0; pass < kPasses; ++pass) {
+      early(pass);
+      if (pass) __syncthreads();
 #pragma unroll
-    for (int jj = 0; jj < R::kAtOnce; ++jj)
+      for (int jj = 0; jj < kAtOnce; ++jj)
 #pragma unroll
-      for (int i = 0; i < SP; ++i)
+        for (int i = 0; i < SP; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const f32x16& a = acc[i][pass * R::kAtOnce + jj];
-          *reinterpret_cast<f32x4*>(lds + (wq * (32 * R::kAtOnce) + jj * 32 + r) * R::kStride + pos(i) + 8 * k + 4 * hh) =
-              f32x4{a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]};
-        }
-    __syncthreads();
-    static_assert(kRounds % GROUP == 0, "whole groups");
-#pragma unroll 1
-    for (int n = 0; n < kRounds; n += GROUP) {
-#pragma unroll
-      for (int i = 0; i < GROUP; ++i) {
-        const int row = first + (n + i) * kPerRound;
-        body(lds + row * R::kStride, q_of(row), col, i);
-      }
-      next();
+          for (int k = 0; k < 4; ++k) {
+            const f32x16& a = acc[i][pass * kAtOnce + jj];
+            *reinterpret_cast<f32x4*>(lds + (wq * kHalf + jj * 32 + r) * kStride + pos(i) + 8 * k + 4 * hh) =
+                f32x4{a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]};
+          }
+      __syncthreads();
+#pragma unroll UNROLL
+      for (int i = 0; i < kRounds; ++i) round(mine + i * kPerRound * kStride, q_of(pass, i), i);
     }
+  }
+};
+
+// four values to memory, bfloat16 with one conversion per pair
+template <typename T>
+__device__ __forceinline__ void put4(T* p, f32x4 v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 a = __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2), b = __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2);
+    *reinterpret_cast<u32x2*>(p) = u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+  } else {
+    *reinterpret_cast<f32x4*>(p) = v;
   }
 }
 
