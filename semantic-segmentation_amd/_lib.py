@@ -181,6 +181,12 @@ _PROTOS = {
     "ssmi_act8_store": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
     "ssmi_act8_restore": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
     "ssmi_act8_restore_bn_act": (_i32, [_vp, _vp, _i64, _i32, _i32, _PB, _i32, _vp, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "ssmi_mx4_quantize": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "ssmi_mx4_quantize_kernel": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "ssmi_mx4_dequantize_kernel": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp]),
+    "ssmi_mx4_workspace_bytes": (_sz, [_i64, _i32]),
+    "ssmi_mx4_dense": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
+    "ssmi_mx4_gated": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32] + [_vp] * 7 + [_i64, _vp, _sz, _vp]),
     "ssmi_gated_ff_workspace_bytes": (_sz, [_PG, _i32]),
     "ssmi_gated_ff_fwd": (_i32, [_PG, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssmi_gated_ff_bwd": (_i32, [_PG] + [_vp] * 12 + [_sz, _vp]),
@@ -203,7 +209,7 @@ _PROTOS["ssmi_cast_bf16_to_f32"] = (_i32, [_vp, _vp, _i64, _vp])
 F32, BF16 = 0, 1      # ssmi dtype codes of activation tensors
 
 EXPORTED_SYMBOLS = tuple(_PROTOS.keys())
-_NOT_STATUS = {"ssmi_gated_ff_workspace_bytes", "ssmi_softmax_xent_static_max_pixels", "ssmi_conv2d_bwd_data_bn_bwd_deferred_supported", "ssmi_expand_supported", "ssmi_expand_workspace_bytes", "ssmi_expand_weight_partial_bytes", "ssmi_conv2d_bwd_data_premerge_supported", "ssmi_conv2d_prebn_supported", "ssmi_logits_tconv2x2_xent_supported", "ssmi_profile_bracket_overhead_ms", "ssmi_device_timestamp_khz", "ssmi_last_error", "ssmi_last_kernel", "ssmi_conv2d_fwd_bn_stats_workspace_bytes", "ssmi_conv2d_bwd_data_bn_bwd_workspace_bytes", "ssmi_conv2d_bwd_data_workspace_bytes", "ssmi_conv2d_bwd_data_uses_rotated", "ssmi_conv2d_pack_usage", "ssmi_comm_size", "ssmi_comm_rank", "ssmi_version", "ssmi_conv2d_bwd_weight_workspace_bytes",
+_NOT_STATUS = {"ssmi_mx4_workspace_bytes", "ssmi_gated_ff_workspace_bytes", "ssmi_softmax_xent_static_max_pixels", "ssmi_conv2d_bwd_data_bn_bwd_deferred_supported", "ssmi_expand_supported", "ssmi_expand_workspace_bytes", "ssmi_expand_weight_partial_bytes", "ssmi_conv2d_bwd_data_premerge_supported", "ssmi_conv2d_prebn_supported", "ssmi_logits_tconv2x2_xent_supported", "ssmi_profile_bracket_overhead_ms", "ssmi_device_timestamp_khz", "ssmi_last_error", "ssmi_last_kernel", "ssmi_conv2d_fwd_bn_stats_workspace_bytes", "ssmi_conv2d_bwd_data_bn_bwd_workspace_bytes", "ssmi_conv2d_bwd_data_workspace_bytes", "ssmi_conv2d_bwd_data_uses_rotated", "ssmi_conv2d_pack_usage", "ssmi_comm_size", "ssmi_comm_rank", "ssmi_version", "ssmi_conv2d_bwd_weight_workspace_bytes",
                "ssmi_conv2d_transpose_bwd_weight_workspace_bytes", "ssmi_bn_workspace_bytes", "ssmi_merge_workspace_bytes",
                "ssmi_softmax_xent_workspace_bytes", "ssmi_mt_consistency_workspace_bytes", "ssmi_superpixel_workspace_bytes"}
 

@@ -8,73 +8,13 @@
 // then  dx = dg Wg^T + du Wu^T  (one product over 2 f) and  dW = x^T dg, x^T du  (one product over the rows, split into strips whose
 // float32 partial sums are added in a fixed order: results do not depend on the launch).
 // All products run on gemm_tile.h: bfloat16 32x32x16 or float32 32x32x2 matrix instructions, float32 sums throughout.
+#include "gate_act.h"
 #include "gemm_tile.h"
 
 namespace ssmi {
 
-enum { kSwish = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
-
-// exp of the bfloat16 variants: v_exp_f32 on x log2(e), relative error under 2^-20 for |x| < 16 - far below the output's 2^-9; the
-// float32 variants take the library's
-template <typename T>
-__device__ __forceinline__ float gate_exp(float v) {
-  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(v * 1.44269504f);
-  return expf(v);
-}
-template <typename T>
-__device__ __forceinline__ float gate_sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-v));      // exp = inf gives 0
-}
-template <typename T, int ACT>
-__device__ __forceinline__ float gate_act(float g) {
-  if constexpr (ACT == kSwish) return g * gate_sigmoid<T>(g);
-  if constexpr (ACT == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678f));
-  if constexpr (ACT == kRelu) return fmaxf(g, 0.f);
-  return gate_sigmoid<T>(g);
-}
-template <typename T, int ACT>
-__device__ __forceinline__ void gate_act_both(float g, float& a, float& d) {
-  if constexpr (ACT == kSwish) {
-    const float s = gate_sigmoid<T>(g);
-    a = g * s;
-    d = s * (1.f + g * (1.f - s));
-  } else if constexpr (ACT == kGelu) {
-    const float c = 0.5f * (1.f + erff(g * 0.70710678f));
-    a = g * c;
-    d = c + g * 0.39894228f * gate_exp<T>(-0.5f * g * g);
-  } else if constexpr (ACT == kRelu) {
-    a = fmaxf(g, 0.f);
-    d = g > 0.f ? 1.f : 0.f;
-  } else {
-    a = gate_sigmoid<T>(g);
-    d = a * (1.f - a);
-  }
-}
-
-// runs body(integral constant) for the activation: one branch around an epilogue, none inside it
-template <int V> struct ActIs { static constexpr int value = V; };
-template <typename Body>
-__device__ __forceinline__ void with_act(int act, Body body) {
-  if (act == kSwish) body(ActIs<kSwish>{});
-  else if (act == kGelu) body(ActIs<kGelu>{});
-  else if (act == kRelu) body(ActIs<kRelu>{});
-  else body(ActIs<kSigmoid>{});
-}
-
 __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
   return bf ? (float)static_cast<const bf16*>(p)[i] : static_cast<const float*>(p)[i];
-}
-
-// Which (p, q) tile a workgroup takes.  Consecutive workgroups of an XCD walk kGroupQ row tiles under one column tile, then the
-// next column tile: the workgroups of an XCD that run together share a few row tiles and column tiles through its L2
-// (1, 2, 4, 8, 16 measured within 3 % of each other).
-static constexpr int kGroupQ = 4;
-struct TileAt { int p, q; };
-__device__ __forceinline__ TileAt tile_at(unsigned v, unsigned np, unsigned nq) {
-  const unsigned per = kGroupQ * np, grp = v / per, in = v - grp * per;
-  const unsigned gq = min((unsigned)kGroupQ, nq - grp * kGroupQ);
-  // divisions run on the vector unit: back to scalars, the tile's addresses hang on them
-  return {(int)__builtin_amdgcn_readfirstlane(in / gq), (int)__builtin_amdgcn_readfirstlane(grp * kGroupQ + in % gq)};
 }
 
 // Stages and K step of a tile shape, and how many of its workgroups a CU holds (registers and LDS)
@@ -117,28 +57,6 @@ struct GateSides : TileShape<SP, SQ> {
   }
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + 2 * W::kBytes, wq * SQ + j, ks); }
 };
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4], int n, bool vec) {
-  if (vec && n >= 4) {
-    Act<T>::gst4(p, f32x4{v[0], v[1], v[2], v[3]});
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) Act<T>::gst(p + i, v[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void fetch4(const T* p, float (&v)[4], int n, bool vec) {
-  if (vec && n >= 4) {
-    const f32x4 a = Act<T>::gld4(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? Act<T>::gld(p + i) : 0.f;
-  }
-}
 
 template <typename T, int SP, int SQ, bool BWD>
 __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
