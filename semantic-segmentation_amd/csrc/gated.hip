@@ -20,7 +20,7 @@ __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
 // Stages and K step of a tile shape, and how many of its workgroups a CU holds (registers and LDS)
 template <int SP, int SQ>
 struct TileShape {
-  static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kPerCu = SP * SQ == 16 ? 1 : 2;
+  static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kPerCu = SP * SQ == 16 ? 1 : SQ == 1 ? 3 : 2;
 };
 
 struct GateArgs {
@@ -31,6 +31,8 @@ struct GateArgs {
   int64_t rows, x_ld, w_ld, out_ld, dy_ld;
   int c, f, fp;                 // fp: units with the padding that [dg | du] rows have
   int act, bf_params, vec_out, vec_dy;
+  int split;                    // backward: [dg | du] as two bfloat16 terms each, [dg | du | rest of dg | rest of du]
+  float* db;                    // backward: column sums of [dg | du] per row tile, or nullptr
   unsigned np, nq;
 };
 
@@ -96,6 +98,23 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(
   T* const out = static_cast<T*>(a.out) + m0 * a.out_ld + f0;
   const T* const dyt = static_cast<const T*>(a.dy) + (BWD ? m0 * a.dy_ld + f0 : 0);
   const unsigned o_lane = (unsigned)R::first() * (unsigned)a.out_ld + (unsigned)col, d_lane = (unsigned)R::first() * (unsigned)a.dy_ld + (unsigned)col;
+  float sum[BWD ? 8 : 1] = {};
+  // [dg | du] of four units of a pixel; with `split` the parts that bfloat16 leaves behind follow
+  auto put_gradients = [&](T* d, const float (&o)[4], const float (&v)[4]) __attribute__((always_inline)) {
+    if constexpr (BWD) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { sum[e] += o[e]; sum[4 + e] += v[e]; }
+      put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
+      put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
+      if (sizeof(T) == 2 && a.split) {
+        f32x4 ro, rv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { ro[e] = o[e] - (float)(T)o[e]; rv[e] = v[e] - (float)(T)v[e]; }
+        put4<T>(d + 2 * a.fp, ro);
+        put4<T>(d + 3 * a.fp, rv);
+      }
+    }
+  };
   with_act(a.act, [&](auto which) __attribute__((always_inline)) {
     constexpr int kAct = decltype(which)::value;
     auto forward = [&](const float* row, float (&o)[4]) __attribute__((always_inline)) {
@@ -128,13 +147,13 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(
             T* const d = out + qc * a.out_ld + o_lane;
             if constexpr (!BWD) {
               forward(row, o);
+              put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
             } else {
               const f32x4 y = Act<T>::up4(dy[i]);
               const float y4[4] = {y[0], y[1], y[2], y[3]};
               backward(row, y4, o, v);
-              put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
+              put_gradients(d, o, v);
             }
-            put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
           });
     } else {
       R::template run<1>(
@@ -156,20 +175,36 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(
                 o[e] = e < n ? o[e] : 0.f;
                 v[e] = e < n ? v[e] : 0.f;
               }
-              put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
-              put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
+              put_gradients(d, o, v);
             }
           });
     }
   });
+  if constexpr (BWD) {
+    if (a.db) {      // the tile's column sums, of the unrounded values: over the threads that share the units, then a row per tile
+      float* const sh = reinterpret_cast<float*>(smem);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sh[((e >> 2) * R::kPerRound + R::first()) * S::kHalf + col + (e & 3)] = sum[e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * S::kHalf; i += 256) {
+        const int side = i / S::kHalf, unit = i - side * S::kHalf;
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < R::kPerRound; ++k) t += sh[(side * R::kPerRound + k) * S::kHalf + unit];
+        if (f0 + unit < a.fp) a.db[(int64_t)at.q * (2 * (int64_t)a.fp) + side * a.fp + f0 + unit] = t;
+      }
+    }
+  }
 }
 
-// dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection
+// dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection (and again
+// over the second terms of a split [dg | du])
 struct GateDxArgs {
   const void *dgu, *wg, *wu;
   void* dx;
   int64_t rows, w_ld, dx_ld;
-  int c, fp, vec_out;
+  int c, fp, vec_out, sides;      // sides: 2, or 4 when split
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
@@ -185,13 +220,12 @@ struct DxSides : TileShape<SP, SQ> {
   typename D::Reader rd;
   int fp, half, wp, wq;
   __device__ __forceinline__ void request(lds_bytes s, int t) const {
-    const bool second = t >= half;
-    const int ts = second ? t - half : t, left = fp - ts * W::kStepK;
+    const int side = t >= 2 * half ? (t >= 3 * half ? 3 : 2) : t >= half ? 1 : 0;
+    const int ts = t - side * half, left = fp - ts * W::kStepK;
     W w = wg;
-    D e = d;
-    if (second) w.rsrc = wu;
+    if (side & 1) w.rsrc = wu;
     w.request(s, ts, left);
-    e.request(s + W::kBytes, ts, left, second ? (unsigned)(fp * (int)sizeof(T)) : 0u);
+    d.request(s + W::kBytes, ts, left, (unsigned)(side * fp * (int)sizeof(T)));
   }
   __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rw.get(s, wp * SP + i, ks); }
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rd.get(s + W::kBytes, wq * SQ + j, ks); }
@@ -211,11 +245,11 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dx_kern
   s.wq = wave & 1;
   s.wg.init(static_cast<const T*>(a.wg) + c0 * a.w_ld, a.w_ld, a.c - c0);
   s.wu = make_rsrc(static_cast<const T*>(a.wu) + c0 * a.w_ld, 0x7FFFFFFFu);
-  s.d.init(static_cast<const T*>(a.dgu) + m0 * (2 * (int64_t)a.fp), 2 * (int64_t)a.fp, (int)min((int64_t)(SQ * 64), a.rows - m0));
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (a.sides * (int64_t)a.fp), a.sides * (int64_t)a.fp, (int)min((int64_t)(SQ * 64), a.rows - m0));
   s.rw.init(lane);
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
-  tile_product<T, SP, SQ>(s, (lds_bytes)smem, 2 * s.half, acc);
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, a.sides * s.half, acc);
   typedef TileRows<SP, SQ, SP * 64> R;
   const int wp = s.wp, c = c0 + R::col();
   auto pos = [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; };
@@ -236,12 +270,12 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dx_kern
   }
 }
 
-// part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]
+// part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]; a split [dg | du] goes through the rows twice
 struct GateDwArgs {
   const void *x, *dgu;
   float* part;
   int64_t rows, x_ld, strip_rows;
-  int c, cp, fp;                // cp: channels with the padding of x rows
+  int c, cp, fp, sides;         // cp: channels with the padding of x rows
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
@@ -254,11 +288,13 @@ struct DwSides : TileShape<SP, SQ> {
   X x;
   typename D::Reader rd;
   typename X::Reader rx;
-  int rows, wp, wq;
+  int rows, once, wp, wq;
+  unsigned second;      // bytes from the first terms of a row to the second ones
   __device__ __forceinline__ void request(lds_bytes s, int t) const {
-    const int left = rows - t * D::kStepK;
-    d.request(s, t, left);
-    x.request(s + D::kBytes, t, left);
+    const bool again = t >= once;
+    const int ts = again ? t - once : t, left = rows - ts * D::kStepK;
+    d.request(s, ts, left, again ? second : 0u);
+    x.request(s + D::kBytes, ts, left);
   }
   __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rd.get(s, wp * SP + i, ks); }
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + D::kBytes, wq * SQ + j, ks); }
@@ -276,12 +312,14 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dw_kern
   s.rows = (int)min(a.strip_rows, a.rows - m0);
   s.wp = wave >> 1;
   s.wq = wave & 1;
-  s.d.init(static_cast<const T*>(a.dgu) + m0 * (2 * (int64_t)a.fp) + p0, 2 * (int64_t)a.fp, 2 * a.fp - p0);
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (a.sides * (int64_t)a.fp) + p0, a.sides * (int64_t)a.fp, 2 * a.fp - p0);
+  s.once = (s.rows + S::D::kStepK - 1) / S::D::kStepK;
+  s.second = 2u * (unsigned)a.fp * (unsigned)sizeof(T);
   s.x.init(static_cast<const T*>(a.x) + m0 * a.x_ld + c0, a.x_ld, a.cp - c0);
   s.rd.init(lane);
   s.rx.init(lane);
   f32x16 acc[SP][SQ];
-  tile_product<T, SP, SQ>(s, (lds_bytes)smem, (s.rows + S::D::kStepK - 1) / S::D::kStepK, acc);
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.sides / 2) * s.once, acc);
   typedef TileRows<SP, SQ, SP * 64> R;
   const int wp = s.wp, p = p0 + R::col();
   float* const part = a.part + ((int64_t)strip * a.c + c0 + R::first()) * (2 * (int64_t)a.fp) + p;
@@ -291,66 +329,65 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dw_kern
                               });
 }
 
-// dW = sum of the strips' partial sums, in their order; four units a thread
-__global__ __launch_bounds__(256) void gate_dw_reduce(const float* __restrict__ part, int strips, int64_t c, int f, int fp, void* dwg, void* dwu, int bf) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // one of c * 2 fp / 4
-  const int quads = fp / 2;
-  if (i >= c * quads) return;
+// dW = sum of the strips' partial sums in their order, db = that of the row tiles' column sums; four units a thread, the bias row last
+struct ReduceArgs {
+  const float *part, *db;
+  void *dwg, *dwu, *dbg, *dbu;
+  int64_t c;
+  int strips, db_tiles, f, fp, bf;
+};
+__global__ __launch_bounds__(256) void gate_reduce_kernel(ReduceArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int quads = a.fp / 2;
   const int64_t ci = i / quads;
   const int p = (int)(i - ci * quads) * 4;
-  const float* s = part + ci * (2 * (int64_t)fp) + p;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  const int64_t step = c * 2 * fp;
-  for (int k = 0; k < strips; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
-  const int fu = p < fp ? p : p - fp;
-  void* const dst = p < fp ? dwg : dwu;
+  const bool bias = ci == a.c;
+  if (ci > a.c || (bias && !a.db)) return;
+  const int fu = p < a.fp ? p : p - a.fp;
+  char* const dst = static_cast<char*>(bias ? (p < a.fp ? a.dbg : a.dbu) : (p < a.fp ? a.dwg : a.dwu));
   if (!dst) return;
+  const int n = bias ? a.db_tiles : a.strips;
+  const int64_t step = (bias ? 1 : a.c) * 2 * a.fp;
+  const float* s = bias ? a.db + p : a.part + ci * (2 * (int64_t)a.fp) + p;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  int k = 0;
+  for (; k + 8 <= n; k += 8) {      // eight on their way at a time
+    f32x4 v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[e];
+  }
+  for (; k < n; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
+  const int64_t at = (bias ? 0 : ci * a.f) + fu;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (fu + e < f) {
-      if (bf) static_cast<bf16*>(dst)[ci * f + fu + e] = (bf16)sum[e];
-      else static_cast<float*>(dst)[ci * f + fu + e] = sum[e];
+    if (fu + e < a.f) {
+      if (a.bf) reinterpret_cast<bf16*>(dst)[at + e] = (bf16)sum[e];
+      else reinterpret_cast<float*>(dst)[at + e] = sum[e];
     }
 }
 
-// column sums of [dg | du]: part[block][2 fp], 4 columns a lane, 64 lanes across, 4 row phases
+// memory rows brought to the tile engine's form: activation type, rows of cols_p >= cols values (16-byte multiples), zeros behind.
+// Up to three matrices a launch (x, both kernels), one per blockIdx.y.
+struct PadJob {
+  const void* src;
+  void* dst;
+  int64_t ld, rows;
+  int cols, cols_p, bf;      // bf: the source is bfloat16
+};
+struct PadJobs { PadJob job[3]; };
 template <typename T>
-__global__ __launch_bounds__(256) void gate_db_kernel(const T* __restrict__ dgu, int64_t rows, int64_t strip_rows, int fp, float* __restrict__ part) {
-  __shared__ f32x4 sh[3][64];
-  const int lane = threadIdx.x & 63, ph = threadIdx.x >> 6;
-  const int p = (blockIdx.x * 64 + lane) * 4;
-  const int64_t ld = 2 * (int64_t)fp, m0 = (int64_t)blockIdx.y * strip_rows, m1 = min(rows, m0 + strip_rows);
-  f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-  if (p < 2 * fp) {
-    int64_t m = m0 + ph;
-    for (; m + 4 < m1; m += 8) {
-      s0 += Act<T>::gld4(dgu + m * ld + p);
-      s1 += Act<T>::gld4(dgu + (m + 4) * ld + p);
-    }
-    if (m < m1) s0 += Act<T>::gld4(dgu + m * ld + p);
-  }
-  s0 += s1;
-  if (ph) sh[ph - 1][lane] = s0;
-  __syncthreads();
-  if (!ph && p < 2 * fp) {
-    s0 += sh[0][lane];
-    s0 += sh[1][lane];
-    s0 += sh[2][lane];
-    *reinterpret_cast<f32x4*>(part + blockIdx.y * ld + p) = s0;
-  }
-}
-
-// memory rows brought to the tile engine's form: activation type, rows of cols_p >= cols values (16-byte multiples), zeros behind
-template <typename S, typename T>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const S* __restrict__ src, int64_t ld, int64_t rows, int cols, int cols_p, T* __restrict__ dst) {
-  const int quads = cols_p / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJobs jobs) {
+  const PadJob j = jobs.job[blockIdx.y];
+  const int quads = j.cols_p / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < j.rows * quads; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / quads;
     const int k = (int)(i - r * quads) * 4;
     f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = k + e < cols ? Act<S>::gld(src + r * ld + k + e) : 0.f;
-    Act<T>::gst4(dst + r * cols_p + k, v);
+    for (int e = 0; e < 4; ++e) v[e] = k + e < j.cols ? param_at(j.src, j.bf, r * j.ld + k + e) : 0.f;
+    Act<T>::gst4(static_cast<T*>(j.dst) + r * j.cols_p + k, v);
   }
 }
 
@@ -444,22 +481,32 @@ static constexpr int kRowsKernelChannels = 2048;        // its x rows have to fi
 static inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
+//   gate, dW: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
+//   dx:       256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192, else as above
+enum Tile { kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
+static Tile tile_for(int64_t q, int64_t p, int64_t times = 1) {
+  if (ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
+  return ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
+}
+static Tile tile_for_dx(int64_t rows, int64_t c) {
+  if (c > 128 && ceil_div64(rows, 256) * ceil_div64(c, 256) >= 192) return kTile256x256;
+  const Tile t = tile_for(rows, c);
+  return t == kTile128x256 ? kTile128x128 : t;
+}
+static inline int64_t q_side(Tile t) { return t == kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
+
 struct GatePlan {
   int es, ce;                       // bytes of an activation, activations in 16 bytes
   int fp, cp;
-  bool pad_w, pad_x, big_dx, big_dw;
+  bool pad_w, pad_x;
+  Tile gate_tile, dx_tile, dw_tile;
   int strips;
   int64_t strip_rows;
-  int db_blocks;
-  int64_t db_rows;
+  bool split;                       // [dg | du] in two bfloat16 terms
+  int db_tiles;
   size_t w_bytes, x_bytes, dgu_bytes, part_bytes, db_bytes;
 };
-
-static bool wants_big(int64_t rows_q, int64_t cols_p) {
-  // 256 x 256 tiles read LDS half as often per product; they pay from about one round of the 256 CUs on (both sides measured, see
-  // launch_gate), below it the four times as many 128 x 128 tiles finish earlier
-  return ceil_div64(rows_q, 256) * ceil_div64(cols_p, 256) >= 192;
-}
 
 static GatePlan gate_plan(const ssmi_gated_desc* d) {
   GatePlan p = {};
@@ -467,30 +514,32 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.ce = 16 / p.es;
   p.fp = (int)up_to(d->f, p.ce);
   p.cp = (int)up_to(d->c, p.ce);
+  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f);
+  p.dx_tile = tile_for_dx(d->rows, d->c);
   p.pad_w = p.fp != d->f || d->param_dtype != d->dtype;
   p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
   p.w_bytes = p.pad_w ? 2 * up256((size_t)d->c * p.fp * p.es) : 0;
   p.x_bytes = p.pad_x ? up256((size_t)d->rows * p.cp * p.es) : 0;
-  p.dgu_bytes = up256((size_t)d->rows * 2 * p.fp * p.es);
-  // strips: about two rounds of workgroups, each strip long enough to be worth its partial sums (512 rows) and short enough that
-  // float32 running sums stay within about 2^-24 sqrt(4096) of exact
-  p.big_dw = (int64_t)ceil_div64(2 * p.fp, 256) * ceil_div64(d->c, 256) * ceil_div64(d->rows, 2048) >= 192;
-  const int64_t side = p.big_dw ? 256 : 128;
-  const int64_t tiles = ceil_div64(2 * p.fp, side) * ceil_div64(d->c, side);
-  int64_t strips = ceil_div64(p.big_dw ? 256 : 512, tiles);
-  strips = strips > ceil_div64(d->rows, 4096) ? strips : ceil_div64(d->rows, 4096);
-  const int64_t most = ceil_div64(d->rows, 512);
+  // One bfloat16 of dg and du is off by 2^-9 on average and shows beside the output's own rounding; two are exact to 2^-17 and cost the two
+  // products that read them twice the arithmetic: nothing below 2^27 multiplications, where launches and latency decide (the backward
+  // pass of 102 x 893 -> 391: 45 us either way), half as much time again above (16k x 512 -> 2048: 260 against 430 us).
+  p.split = d->dtype == SSMI_BF16 && (double)d->rows * d->c * d->f <= (double)(1 << 27);
+  p.dgu_bytes = up256((size_t)d->rows * (p.split ? 4 : 2) * p.fp * p.es);
+  // strips of the weight gradient: one round of workgroups (two to a CU), each strip long enough to be worth its partial sums (512 rows)
+  // and, in float32, short enough for the running sums (4096 rows: 2^-24 sqrt(4096) of a term)
+  const int64_t most = ceil_div64(d->rows, 512), least = d->dtype == SSMI_BF16 ? 1 : ceil_div64(d->rows, 4096);
+  // and the larger tile only under strips of 4096 rows, where its own speed outweighs the partial sums of twice the strips
+  const int64_t wide = ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, 256);
+  p.dw_tile = d->c > 128 && d->rows / ceil_div64(512, wide) >= 4096 ? kTile128x256 : tile_for(d->c, 2 * p.fp, most);
+  if (p.dw_tile == kTile128x256 && d->rows / ceil_div64(512, wide) < 4096) p.dw_tile = kTile128x128;
+  int64_t strips = ceil_div64(512, ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, q_side(p.dw_tile)));
   strips = strips < most ? strips : most;
+  strips = strips > least ? strips : least;
   p.strip_rows = up_to(ceil_div64(d->rows, strips), 64);
   p.strips = (int)ceil_div64(d->rows, p.strip_rows);
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
-  const int64_t dbx = ceil_div64(2 * p.fp, 256);
-  int64_t dby = ceil_div64(1024, dbx);
-  const int64_t dbm = ceil_div64(d->rows, 64);
-  dby = dby < dbm ? dby : dbm;
-  p.db_rows = ceil_div64(d->rows, dby);
-  p.db_blocks = (int)ceil_div64(d->rows, p.db_rows);
-  p.db_bytes = up256((size_t)p.db_blocks * 2 * p.fp * 4);
+  p.db_tiles = (int)ceil_div64(d->rows, q_side(p.gate_tile));
+  p.db_bytes = up256((size_t)p.db_tiles * 2 * p.fp * 4);
   return p;
 }
 
@@ -510,12 +559,6 @@ static ssmi_status check_desc(const char* who, const ssmi_gated_desc* d) {
 
 static inline bool aligned(const void* p, int b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
 
-template <typename S, typename T>
-static void pad_rows(const void* src, int64_t ld, int64_t rows, int cols, int cols_p, void* dst, hipStream_t st) {
-  const int64_t n = ceil_div64(rows * (cols_p / 4), 256);
-  hipLaunchKernelGGL((pad_rows_kernel<S, T>), dim3((unsigned)(n < 8192 ? n : 8192)), dim3(256), 0, st, static_cast<const S*>(src), ld, rows, cols, cols_p, static_cast<T*>(dst));
-}
-
 // operands in the tile engine's form, padded copies in ws where they are not in it already
 struct Staged {
   const void *x, *wg, *wu;
@@ -525,26 +568,28 @@ struct Staged {
 template <typename T>
 static Staged stage_operands(const ssmi_gated_desc* d, const GatePlan& p, const void* x, const void* wg, const void* wu, void* ws, hipStream_t st) {
   Staged s = {x, wg, wu, d->x_ld, d->f, static_cast<char*>(ws)};
+  PadJobs jobs = {};
+  int n = 0;
+  int64_t most = 0;
+  auto add = [&](const void* src, int64_t ld, int64_t rows, int cols, int cols_p, bool bf) {
+    jobs.job[n++] = {src, s.ws, ld, rows, cols, cols_p, bf};
+    most = most > rows * (cols_p / 4) ? most : rows * (cols_p / 4);
+    const void* at = s.ws;
+    s.ws += up256((size_t)rows * cols_p * sizeof(T));
+    return at;
+  };
   if (p.pad_w) {
-    const size_t one = p.w_bytes / 2;
-    void *a = s.ws, *b = s.ws + one;
-    if (d->param_dtype == SSMI_BF16) {
-      pad_rows<bf16, T>(wg, d->f, d->c, d->f, p.fp, a, st);
-      pad_rows<bf16, T>(wu, d->f, d->c, d->f, p.fp, b, st);
-    } else {
-      pad_rows<float, T>(wg, d->f, d->c, d->f, p.fp, a, st);
-      pad_rows<float, T>(wu, d->f, d->c, d->f, p.fp, b, st);
-    }
-    s.wg = a;
-    s.wu = b;
+    s.wg = add(wg, d->f, d->c, d->f, p.fp, d->param_dtype == SSMI_BF16);
+    s.wu = add(wu, d->f, d->c, d->f, p.fp, d->param_dtype == SSMI_BF16);
     s.w_ld = p.fp;
-    s.ws += p.w_bytes;
   }
   if (p.pad_x) {
-    pad_rows<T, T>(x, d->x_ld, d->rows, d->c, p.cp, s.ws, st);
-    s.x = s.ws;
+    s.x = add(x, d->x_ld, d->rows, d->c, p.cp, d->dtype == SSMI_BF16);
     s.x_ld = p.cp;
-    s.ws += p.x_bytes;
+  }
+  if (n) {
+    const int64_t blocks = ceil_div64(most, 256);
+    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)n), dim3(256), 0, st, jobs);
   }
   return s;
 }
@@ -562,8 +607,9 @@ static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
   return SSMI_OK;
 }
 template <typename T, bool BWD>
-static ssmi_status launch_gate(const GateArgs& a, hipStream_t st) {
-  return wants_big(a.rows, 2 * (int64_t)a.f) ? launch_gate_as<T, 2, 4, BWD>(a, st) : launch_gate_as<T, 2, 2, BWD>(a, st);
+static ssmi_status launch_gate(Tile t, const GateArgs& a, hipStream_t st) {
+  if (t == kTile128x256) return launch_gate_as<T, 2, 4, BWD>(a, st);
+  return t == kTile128x128 ? launch_gate_as<T, 2, 2, BWD>(a, st) : launch_gate_as<T, 2, 1, BWD>(a, st);
 }
 template <typename T, int SP, int SQ>
 static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
@@ -617,9 +663,10 @@ static ssmi_status gated_fwd(const ssmi_gated_desc* d, const void* x, const void
   }
   const GatePlan p = gate_plan(d);
   const Staged s = stage_operands<T>(d, p, x, wg, wu, ws, st);
+  SSMI_LAUNCH_CHECK();
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.fp = p.fp;
   a.vec_out = d->y_ld % 4 == 0 && aligned(y, 4 * p.es);
-  return launch_gate<T, false>(a, st);
+  return launch_gate<T, false>(p.gate_tile, a, st);
 }
 
 template <typename T>
@@ -633,31 +680,33 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   const int bf = d->param_dtype == SSMI_BF16;
   GateArgs a = {};
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.bg = bg; a.bu = bu; a.dy = dy; a.out = dgu;
-  a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = 2 * (int64_t)p.fp; a.dy_ld = d->y_ld;
-  a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf;
+  SSMI_LAUNCH_CHECK();
+  const int sides = p.split ? 4 : 2;
+  a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = sides * (int64_t)p.fp; a.dy_ld = d->y_ld;
+  a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf; a.split = p.split;
+  a.db = dbg || dbu ? dbp : nullptr;
   a.vec_out = 1;
   a.vec_dy = d->y_ld % 4 == 0 && aligned(dy, 4 * p.es);
-  ssmi_status r = launch_gate<T, true>(a, st);
+  ssmi_status r = launch_gate<T, true>(p.gate_tile, a, st);
   if (r != SSMI_OK) return r;
   if (dx) {
     GateDxArgs b = {};
-    b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp;
+    b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp; b.sides = sides;
     b.vec_out = d->x_ld % 4 == 0 && aligned(dx, 4 * p.es);
-    r = wants_big(d->rows, d->c) ? launch_dx_as<T, 4, 4>(b, st) : launch_dx_as<T, 2, 2>(b, st);
+    r = p.dx_tile == kTile256x256 ? launch_dx_as<T, 4, 4>(b, st) : p.dx_tile == kTile128x128 ? launch_dx_as<T, 2, 2>(b, st) : launch_dx_as<T, 2, 1>(b, st);
     if (r != SSMI_OK) return r;
   }
-  if (dwg || dwu) {
+  const bool dw = dwg || dwu;
+  if (dw) {
     GateDwArgs b = {};
-    b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp;
-    r = p.big_dw ? launch_dw_as<T, 2, 4>(b, p.strips, st) : launch_dw_as<T, 2, 2>(b, p.strips, st);
+    b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp; b.sides = sides;
+    r = p.dw_tile == kTile128x256 ? launch_dw_as<T, 2, 4>(b, p.strips, st) : p.dw_tile == kTile128x128 ? launch_dw_as<T, 2, 2>(b, p.strips, st) : launch_dw_as<T, 2, 1>(b, p.strips, st);
     if (r != SSMI_OK) return r;
-    hipLaunchKernelGGL(gate_dw_reduce, dim3((unsigned)ceil_div64((int64_t)d->c * (p.fp / 2), 256)), dim3(256), 0, st, part, p.strips, (int64_t)d->c, d->f, p.fp, dwg, dwu, bf);
-    SSMI_LAUNCH_CHECK();
   }
-  if (dbg || dbu) {
-    hipLaunchKernelGGL((gate_db_kernel<T>), dim3((unsigned)ceil_div64(2 * p.fp, 256), (unsigned)p.db_blocks), dim3(256), 0, st, static_cast<const T*>(dgu), d->rows, p.db_rows, p.fp, dbp);
-    SSMI_LAUNCH_CHECK();
-    hipLaunchKernelGGL(gate_dw_reduce, dim3((unsigned)ceil_div64(p.fp / 2, 256)), dim3(256), 0, st, dbp, p.db_blocks, (int64_t)1, d->f, p.fp, dbg, dbu, bf);
+  if (dw || a.db) {
+    const ReduceArgs b = {part, a.db, dwg, dwu, dbg, dbu, dw ? d->c : 0, p.strips, p.db_tiles, d->f, p.fp, bf};
+    const int64_t threads = (b.c + (a.db ? 1 : 0)) * (p.fp / 2);
+    hipLaunchKernelGGL(gate_reduce_kernel, dim3((unsigned)ceil_div64(threads, 256)), dim3(256), 0, st, b);
     SSMI_LAUNCH_CHECK();
   }
   return SSMI_OK;

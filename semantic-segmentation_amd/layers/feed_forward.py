@@ -10,6 +10,7 @@ the 4-bit matrix instructions; that form has no backward pass."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -35,13 +36,17 @@ def _aligned_rows(x):
 
 
 def _dense(w):
-    w = w.contiguous()
+    if not w.is_contiguous():
+        w = w.contiguous()
     return w.clone() if w.data_ptr() % 16 else w
 
 
-def _workspace(desc, backward, like):
-    n = lib().gated_ff_workspace_bytes(C.byref(desc), backward)
-    return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
+@functools.lru_cache(maxsize=4096)
+def _plan(rows, x_ld, y_ld, c, f, act, dtype, param_dtype, backward):
+    """The descriptor of a call and its workspace size, by sizes and types alone."""
+    d = GatedDesc(rows, x_ld, y_ld, c, f, act, dtype, param_dtype)
+    ref = C.byref(d)
+    return ref, int(lib().gated_ff_workspace_bytes(ref, backward)), d
 
 
 def _forward(x, wg, wu, bg, bu, act):
@@ -50,51 +55,52 @@ def _forward(x, wg, wu, bg, bu, act):
     y = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
     if not rows:
         return y
-    d = GatedDesc(rows, ld, f, c, f, act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"))
+    ref, n, _ = _plan(rows, ld, f, c, f, act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"), 0)
     with on(x):
-        ws, n = _workspace(d, 0, x)
-        lib().gated_ff_fwd(C.byref(d), t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), y.data_ptr(), _ptr(ws), n, stream_of(x))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        lib().gated_ff_fwd(ref, t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), y.data_ptr(), _ptr(ws), n, stream_of(x))
     return y
 
 
 class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, bg, bu, act, checkpoint):
-        wg, wu, bg, bu = _dense(wg), _dense(wu), None if bg is None else bg.contiguous(), None if bu is None else bu.contiguous()
+        wg, wu = _dense(wg), _dense(wu)
+        if bg is not None:
+            bg, bu = bg.contiguous(), bu.contiguous()
         y = _forward(x, wg, wu, bg, bu, act)
-        ctx.act, ctx.shape, ctx.kept = act, x.shape, None
-        if checkpoint is None or not ctx.needs_input_grad[:5].count(True):
-            ctx.save_for_backward(x, wg, wu, bg, bu)
-        else:
-            ctx.kept = store_8bit(x)
-            ctx.save_for_backward(None, wg, wu, bg, bu)
+        ctx.act = act
+        ctx.kept = None if checkpoint is None else store_8bit(x)
+        ctx.save_for_backward(x if checkpoint is None else None, wg, wu, bg, bu)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():      # create_graph=True: what follows is not recorded
+            raise RuntimeError("gated_feed_forward has no second derivative")
         x, wg, wu, bg, bu = ctx.saved_tensors
         if x is None:
             x = ctx.kept.restore()
-        need = ctx.needs_input_grad
+        nx, ng, nu, nbg, nbu = ctx.needs_input_grad[:5]
         c, f = wg.shape
         t, rows, ld = _aligned_rows(x)
         if not rows:
-            return (torch.zeros_like(x) if need[0] else None, *(torch.zeros_like(p) if n else None for p, n in zip((wg, wu, bg, bu), need[1:5])), None, None)
+            return (torch.zeros_like(x) if nx else None, *(torch.zeros_like(p) if n else None for p, n in ((wg, ng), (wu, nu), (bg, nbg), (bu, nbu))), None, None)
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
         dt, _, dy_ld = rows_of(dy)
-        dx = None
-        if need[0]:      # the row stride of dx is that of x
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if ld != c:
-                t, ld = _dense(t), c
-        dwg, dwu, dbg, dbu = (torch.empty_like(p) if n else None for p, n in zip((wg, wu, bg, bu), need[1:5]))
-        d = GatedDesc(rows, ld, dy_ld, c, f, ctx.act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"))
+        if nx and ld != c:      # the row stride of dx is that of x
+            t, ld = _dense(t), c
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if nx else None
+        dwg = torch.empty_like(wg) if ng else None
+        dwu = torch.empty_like(wu) if nu else None
+        dbg = torch.empty_like(bg) if nbg else None
+        dbu = torch.empty_like(bu) if nbu else None
+        ref, n, _ = _plan(rows, ld, dy_ld, c, f, ctx.act, dtype_code(x, "gated_feed_forward"), dtype_code(wg, "gated_feed_forward"), 1)
         with on(x):
-            ws, n = _workspace(d, 1, x)
-            lib().gated_ff_bwd(C.byref(d), t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), dt.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu),
-                               _ptr(dbg), _ptr(dbu), _ptr(ws), n, stream_of(x))
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            lib().gated_ff_bwd(ref, t.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), dt.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu),
+                               _ptr(dbg), _ptr(dbu), ws.data_ptr(), n, stream_of(x))
         return dx, dwg, dwu, dbg, dbu, None, None
 
 
@@ -118,16 +124,21 @@ def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="swis
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[0] != x.shape[-1] or 0 in w_gate.shape:
         raise ValueError("{}: kernels must both be [{}, units], got {} and {}".format(who, x.shape[-1] if x.dim() else "channels", tuple(w_gate.shape), tuple(w_up.shape)))
     f = w_gate.shape[1]
-    params = [w_gate, w_up] + ([] if b_gate is None else [b_gate, b_up])
+    params = (w_gate, w_up) if b_gate is None else (w_gate, w_up, b_gate, b_up)
+    dev, pt = x.device, w_gate.dtype
+    learns = x.requires_grad
     for p in params:
-        if p.device != x.device or p.dtype != w_gate.dtype or not (p.dtype == torch.float32 or (p.dtype == torch.bfloat16 and code == BF16)):
-            raise ValueError("{}: parameters must be float32 (or all bfloat16 under a bfloat16 input) on {}".format(who, x.device))
+        if p.dtype != pt or p.device != dev or not (pt == torch.float32 or (pt == torch.bfloat16 and code == BF16)):
+            raise ValueError("{}: parameters must be float32 (or all bfloat16 under a bfloat16 input) on {}".format(who, dev))
+        learns = learns or p.requires_grad
     if b_gate is not None and (b_gate.shape != (f,) or b_up.shape != (f,)):
         raise ValueError("{}: biases must be [{}], got {} and {}".format(who, f, tuple(b_gate.shape), tuple(b_up.shape)))
-    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+    if learns and torch.is_grad_enabled():
         return _GatedFn.apply(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation], checkpoint)
-    return _forward(x.detach(), _dense(w_gate.detach()), _dense(w_up.detach()), None if b_gate is None else b_gate.detach().contiguous(),
-                    None if b_up is None else b_up.detach().contiguous(), ACTIVATIONS[activation])
+    with torch.no_grad():
+        if b_gate is not None:
+            b_gate, b_up = b_gate.contiguous(), b_up.contiguous()
+        return _forward(x, _dense(w_gate), _dense(w_up), b_gate, b_up, ACTIVATIONS[activation])
 
 
 class GatedFeedForward2D(object):

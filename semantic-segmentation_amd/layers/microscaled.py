@@ -8,6 +8,8 @@ include/ssmi.h states the format).  Weights are quantised once, inputs inside th
 These calls have no backward pass."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .._lib import lib
@@ -76,8 +78,13 @@ def _operand(x, w: MX4Weights, who):
     return t, rows, ld, torch.empty(x.shape[:-1] + (w.n,), dtype=x.dtype, device=x.device)
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows, k):
+    return int(lib().mx4_workspace_bytes(rows, k))
+
+
 def _workspace(rows, k, like):
-    n = lib().mx4_workspace_bytes(rows, k)
+    n = _workspace_bytes(rows, k)
     return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
 
 
