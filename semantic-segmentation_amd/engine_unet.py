@@ -7,9 +7,15 @@ check, never a padded copy) and one fused BN + LeakyReLU + dropout pass; the bac
 UpSampling2D + concatenate (src/models.py:920-927) never materialise separately: the upsampling kernel and the skip copy
 write the two channel slices of one buffer, and the gradient of the skip slice is added straight from the decoder's
 gradient buffer when the encoder block runs its backward.
+
+With `activation_checkpoints="8bit"` a block keeps its raw convolution outputs as 8-bit checkpoints (ssmi_act8_*) instead of two
+activation tensors per convolution block: everything else that only waits for the backward pass, and every gradient that only travels
+to the next launch, lives in seven buffers that all blocks share (`Scratch`).  The forward pass is unchanged bit for bit; the backward
+pass sees the restored convolution outputs, and the block outputs formed from them.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Dict, List, Optional
 
 import torch
@@ -20,6 +26,32 @@ from .engine import (ACT_LEAKY, ACT_NONE, BatchNorm, Block, ClassifierHead, Conv
 
 DROP_RATE = 0.1     # src/models.py:841
 LEAKY_ALPHA = 0.1   # src/models.py:840
+
+
+class Scratch:
+    """What the convolution blocks of a graph with 8-bit checkpoints share.  All of its work runs on one stream (the graph keeps its
+    weight gradients on the main stream), so a buffer is free again as soon as the launches that read it are queued.
+      y        the raw convolution output of the block at work; in the backward pass the restored one
+      x        backward pass: the restored output of the block in front (operand of the weight gradient)
+      out[2]   outputs of blocks inside a run, in turn: the inference phase reads one while it writes the other
+      dy[2]    gradients at the raw outputs of a block and of the block in front of it
+      da       the data gradient between the two"""
+
+    def __init__(self):
+        self.size = 0
+        self.buf = None
+
+    def need(self, values: int) -> None:
+        self.size = max(self.size, (values + 63) // 64 * 64)      # every buffer starts 16-byte aligned
+
+    def plan(self, dtype, dev) -> None:
+        self.buf = torch.empty(7, self.size, dtype=dtype, device=dev)
+
+    def view(self, k: int, shape) -> torch.Tensor:
+        n = 1
+        for d in shape:
+            n *= d
+        return self.buf[k, :n].view(shape)
 
 
 class ConvUnit:
@@ -35,16 +67,47 @@ class ConvUnit:
         self.drop_name = name + "_dropout"
         self.drop_mask = None
         self.needs_dx = True
+        self.scratch: Optional[Scratch] = None      # 8-bit checkpoints: the graph's shared buffers
+        self.first, self.last, self.turn = True, True, 0      # place in its run of blocks, and in the graph
 
     def plan(self, n, h, w, dev, x_ld=None):
         f32 = dict(dtype=self.store.act_dtype, device=dev)      # activation type
         self.n, self.h, self.w, self.npix = n, h, w, n * h * w
         self.conv.plan(n, h, w, x_ld=x_ld)
         self.bn.plan(dev)
+        if self.scratch is not None:
+            # kept: the checkpoint; the output where another block reads it later, the input gradient where it leaves the run
+            self.codes = torch.empty(self.npix, self.cout, dtype=torch.uint8, device=dev)
+            self.scales = torch.empty(self.npix, (self.cout + 31) // 32, dtype=torch.uint8, device=dev)
+            self.out = torch.empty(n, h, w, self.cout, **f32) if self.last else None
+            self.dx = torch.empty(n, h, w, self.cin, **f32) if self.needs_dx and self.first else None
+            self.scratch.need(self.npix * (self.cout if self.first else max(self.cout, self.cin)))
+            return
         self.y = torch.empty(n, h, w, self.cout, **f32)
         self.out = torch.empty_like(self.y)
         self.dy = torch.empty_like(self.y)
         self.dx = torch.empty(n, h, w, self.cin, **f32) if self.needs_dx else None
+
+    def bind_scratch(self):
+        """Views of the shared buffers, once all blocks have said how large they have to be."""
+        s = self.scratch
+        shape, xshape = (self.n, self.h, self.w, self.cout), (self.n, self.h, self.w, self.cin)
+        self.y, self.dy = s.view(0, shape), s.view(4 + self.turn % 2, shape)
+        self.restored_out = s.view(1, shape)
+        if not self.last:
+            self.out = s.view(2 + self.turn % 2, shape)
+        if self.needs_dx and not self.first:
+            self.dx = s.view(6, xshape)
+
+    def restore(self, cfg: RunCfg, with_out: bool):
+        """8-bit checkpoints: `y` and, with_out, the block's output as the backward pass sees them."""
+        bn = self.bn
+        if not with_out:
+            lib().act8_restore(_ptr(self.codes), _ptr(self.scales), self.npix, self.cout, self.store.dtype_code, _ptr(self.y), self.cout, cfg.st)
+            return
+        drop = self.drop_mask if cfg.use_dropout else None
+        lib().act8_restore_bn_act(_ptr(self.codes), _ptr(self.scales), self.npix, self.cout, self.store.dtype_code, C.byref(bn.params), self.act, None,
+                                  LEAKY_ALPHA, _ptr(drop), self.h * self.w, _ptr(self.y), self.cout, _ptr(self.restored_out), self.cout, cfg.st)
 
     def fwd(self, x, cfg: RunCfg):
         L = self.store.L
@@ -54,6 +117,8 @@ class ConvUnit:
             self.conv.fwd_bn_act_infer(x, self.out, bn, cfg.st, act=self.act, slope=LEAKY_ALPHA)
             return self.out
         self.conv.fwd_bn(x, self.y, bn, self.npix, cfg.training, cfg.update_moving, cfg.unbiased_moving, cfg.ws, cfg.st)
+        if self.scratch is not None and cfg.training:
+            lib().act8_store(_ptr(self.y), self.cout, self.npix, self.cout, self.store.dtype_code, _ptr(self.codes), _ptr(self.scales), cfg.st)
         drop = self.drop_mask if cfg.use_dropout else None
         L.bn_act_drop_fwd(_ptr(self.y), self.cout, _ptr(bn.mean), _ptr(bn.invstd), _ptr(bn.gamma), _ptr(bn.beta), self.act,
                           None, LEAKY_ALPHA, _ptr(drop), self.h * self.w, _ptr(self.out), self.cout, self.npix, self.cout,
@@ -65,6 +130,8 @@ class ConvUnit:
         the raw convolution output) and the BN parameter gradients."""
         L = self.store.L
         bn = self.bn
+        if self.scratch is not None:
+            self.restore(cfg, with_out=False)
         drop = self.drop_mask if cfg.use_dropout else None
         L.bn_act_drop_bwd(dout_ptr, dout_ld, _ptr(self.y), self.cout, _ptr(bn.mean), _ptr(bn.invstd), _ptr(bn.gamma),
                           _ptr(bn.beta), self.act, None, LEAKY_ALPHA, _ptr(drop), self.h * self.w, _ptr(self.dy),
@@ -75,7 +142,11 @@ class ConvUnit:
         """Weight gradient and data gradient of the convolution from self.dy.  With `producer` (the unit whose output is
         this unit's input) the data gradient and the producer's BN backward run as one fused call and land in
         producer.dy; returns dx otherwise (None when the input needs no gradient)."""
-        cfg.wgrad(self.conv, self.x, self.dy)
+        x = self.x
+        if producer is not None and self.scratch is not None:
+            producer.restore(cfg, with_out=True)
+            x = producer.restored_out
+        cfg.wgrad(self.conv, x, self.dy)
         if producer is not None:
             p = producer
             drop = p.drop_mask if cfg.use_dropout else None
@@ -275,8 +346,9 @@ SEGNET = dict(
 class UNetSegNetGraph(GraphBase):
     """`unet` / `segnet`: four encoder blocks, (U-Net) the connecting block, four decoder blocks, 1x1 logits."""
 
-    def __init__(self, kind: str, num_classes: int, device="cuda", encoder_only: bool = False, act_dtype=torch.float32):
-        assert kind in ("unet", "segnet")
+    def __init__(self, kind: str, num_classes: int, device="cuda", encoder_only: bool = False, act_dtype=torch.float32,
+                 activation_checkpoints: Optional[str] = None):
+        assert kind in ("unet", "segnet") and activation_checkpoints in (None, "8bit")
         assert not (encoder_only and kind == "unet")      # the reference has no unet-encoder-only
         topo = UNET if kind == "unet" else SEGNET
         self.variant, self.num_classes, self.encoder_only = kind, num_classes, encoder_only
@@ -291,7 +363,7 @@ class UNetSegNetGraph(GraphBase):
         blocks.extend(encs)
         if encoder_only:      # src/models.py:985-993: average pooling over pool4 -> Flatten -> Dense
             blocks.append(ClassifierHead(st, c, num_classes))
-            self._finish_init(blocks)
+            self._finish_blocks(blocks, activation_checkpoints)
             return
         if topo["connect"]:
             cb = ConnectingBlock(st, topo["connect"], c)
@@ -301,9 +373,32 @@ class UNetSegNetGraph(GraphBase):
             blocks.append(DecoderBlock(st, prefix, n, c, encs[skip], f))
             c = f
         blocks.append(PointwiseHead(st, c, num_classes))
+        self._finish_blocks(blocks, activation_checkpoints)
+
+    def _finish_blocks(self, blocks, activation_checkpoints):
         self._finish_init(blocks)
+        self.checkpointed = []
+        if activation_checkpoints is None:
+            return
+        self.overlap_weight_gradients = False      # the shared buffers live on one stream
+        turn = 0
+        for b in blocks:
+            if not isinstance(b, UnitBlock):
+                continue
+            for u in b.units:
+                u.first, u.last, u.turn = u is b.units[0], u is b.units[-1], turn
+                self.checkpointed.append(u)
+                turn += 1
 
     def _plan_blocks(self, n, h, w, dev):
+        if self.checkpointed:
+            scratch = Scratch()
+            for u in self.checkpointed:
+                u.scratch = scratch
         hh, ww = h, w
         for b in self.blocks:
             hh, ww, _ = b.plan(n, hh, ww, dev)
+        if self.checkpointed:
+            scratch.plan(self.store.act_dtype, dev)
+            for u in self.checkpointed:
+                u.bind_scratch()

@@ -60,11 +60,20 @@ def _norm_index(idx, n):
 class ModelBase(object):
     """src/models.py:157-205."""
 
+    _takes_checkpoints = False
+
     def __init__(self, name, input_shape, num_classes, model_lambda_loss_type=ModelLambdaLossType.NONE, device="cuda",
-                 dtype="f32"):
+                 dtype="f32", activation_checkpoints=None):
         """`dtype` (no counterpart in the reference, which is float32 only): element type of the activation tensors in
-        device memory, "f32" or "bf16".  Parameters, statistics, optimizer state and arithmetic are float32 either way."""
+        device memory, "f32" or "bf16".  Parameters, statistics, optimizer state and arithmetic are float32 either way.
+        `activation_checkpoints` ("8bit" or None; U-Net and SegNet): keep the convolution outputs in 8 bits for the backward
+        pass.  Outputs and losses are unchanged, gradients are those at the restored activations."""
         import torch
+        if activation_checkpoints not in (None, "8bit"):
+            raise ValueError('Unknown activation checkpoints: {} (expected None or "8bit")'.format(activation_checkpoints))
+        if activation_checkpoints is not None and not self._takes_checkpoints:
+            raise ValueError('{} keeps its activations as they are: activation_checkpoints is for the U-Net and SegNet models'.format(name))
+        self.activation_checkpoints = activation_checkpoints
         try:
             self.act_dtype = {"f32": torch.float32, "float32": torch.float32, torch.float32: torch.float32,
                               "bf16": torch.bfloat16, "bfloat16": torch.bfloat16, torch.bfloat16: torch.bfloat16}[dtype]
@@ -243,15 +252,20 @@ class ENetNaiveUpsamplingEnhanced(ModelBase):
 class UNetModel(ModelBase):
     """src/models.py:771-943."""
 
+    _takes_checkpoints = True
+
     def __init__(self, input_shape, num_classes, model_lambda_loss_type=ModelLambdaLossType.NONE, **kw):
         super().__init__("UNet", input_shape, num_classes, model_lambda_loss_type, **kw)
 
     def _build_model(self):
-        return UNetSegNetGraph("unet", self.num_classes, self.device, act_dtype=self.act_dtype)
+        return UNetSegNetGraph("unet", self.num_classes, self.device, act_dtype=self.act_dtype,
+                               activation_checkpoints=self.activation_checkpoints)
 
 
 class SegNetBasicModel(ModelBase):
     """src/models.py:951-1012."""
+
+    _takes_checkpoints = True
 
     def __init__(self, input_shape, num_classes, encoder_only=False, model_lambda_loss_type=ModelLambdaLossType.NONE, **kw):
         self.encoder_only = encoder_only
@@ -259,7 +273,8 @@ class SegNetBasicModel(ModelBase):
                          model_lambda_loss_type, **kw)
 
     def _build_model(self):
-        return UNetSegNetGraph("segnet", self.num_classes, self.device, encoder_only=self.encoder_only, act_dtype=self.act_dtype)
+        return UNetSegNetGraph("segnet", self.num_classes, self.device, encoder_only=self.encoder_only, act_dtype=self.act_dtype,
+                               activation_checkpoints=self.activation_checkpoints)
 
 
 def get_model(model_name, input_shape, num_classes, model_lambda_loss_type=ModelLambdaLossType.NONE, **kw):

@@ -238,8 +238,9 @@ class SegmentationTrainer(object):
                  (True, True): T.SEGMENTATION_SEMI_SUPERVISED_MEAN_TEACHER_SUPERPIXEL}[(self.using_mean_teacher_method,
                                                                                           self.using_superpixel_method)]
         # "activation_dtype": "f32" (default) | "bf16": storage format of activations and their gradients in HBM
+        # "activation_checkpoints": null (default) | "8bit": U-Net / SegNet keep what waits for the backward pass in 8 bits
         mb = models.get_model(model_name, tuple(config.get("input_shape", [None, None, 3])), num_classes, ltype, device=self.device,
-                              dtype=config.get("activation_dtype", "f32"))
+                              dtype=config.get("activation_dtype", "f32"), activation_checkpoints=config.get("activation_checkpoints"))
         self.model_wrapper = mb
         self.model = mb.model
         self.model.seed = self.random_seed + self.rank   # independent dropout draws per replica
