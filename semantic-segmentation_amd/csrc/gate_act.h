@@ -17,11 +17,29 @@ template <typename T>
 __device__ __forceinline__ float gate_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-v));      // exp = inf gives 0
 }
+// Phi(g) = (1 + erf(g / sqrt 2)) / 2, and exp(-g^2 / 2) beside it.  bfloat16: Abramowitz and Stegun 7.1.26, whose own exponential is the
+// density's - erf off by at most 1.5e-7, one reciprocal, one exponential, seven multiply-adds (the library's erff costs four times that
+// and the registers of both its branches); float32: the library's.
+template <typename T>
+__device__ __forceinline__ float gate_phi(float g, float& density) {
+  density = gate_exp<T>(-0.5f * g * g);
+  if constexpr (sizeof(T) == 2) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(g), 1.f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float upper = 0.5f * p * t * density;      // 1 - Phi(|g|)
+    return g < 0.f ? upper : 1.f - upper;
+  }
+  return 0.5f * (1.f + erff(g * 0.70710678f));
+}
 template <typename T, int ACT>
 __device__ __forceinline__ float gate_act(float g) {
+  [[maybe_unused]] float density;
   if constexpr (ACT == kSwish) return g * gate_sigmoid<T>(g);
-  if constexpr (ACT == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678f));
-  if constexpr (ACT == kRelu) return fmaxf(g, 0.f);
+  if constexpr (ACT == kGelu) return g * gate_phi<T>(g, density);
+  if constexpr (ACT == kRelu) return g < 0.f ? 0.f : g;      // a NaN stays one
   return gate_sigmoid<T>(g);
 }
 template <typename T, int ACT>
@@ -31,11 +49,12 @@ __device__ __forceinline__ void gate_act_both(float g, float& a, float& d) {
     a = g * s;
     d = s * (1.f + g * (1.f - s));
   } else if constexpr (ACT == kGelu) {
-    const float c = 0.5f * (1.f + erff(g * 0.70710678f));
+    float density;
+    const float c = gate_phi<T>(g, density);
     a = g * c;
-    d = c + g * 0.39894228f * gate_exp<T>(-0.5f * g * g);
+    d = c + g * 0.39894228f * density;
   } else if constexpr (ACT == kRelu) {
-    a = fmaxf(g, 0.f);
+    a = g < 0.f ? 0.f : g;
     d = g > 0.f ? 1.f : 0.f;
   } else {
     a = gate_sigmoid<T>(g);

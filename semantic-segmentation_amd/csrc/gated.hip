@@ -17,10 +17,18 @@ __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
   return bf ? (float)static_cast<const bf16*>(p)[i] : static_cast<const float*>(p)[i];
 }
 
-// Stages and K step of a tile shape, and how many of its workgroups a CU holds (registers and LDS)
+// Stages, K step, q rows that the epilogue takes at once and workgroups to a CU (registers and LDS) of a tile shape.  The products of dx
+// and dW run long K loops: 128-byte steps, fewer barriers (16k x 512 -> 2048: dx 65 us, with 64-byte steps 92).  The gate kernels run
+// short ones with an epilogue as long: the 128 x 128 tile takes 64-byte steps and a quarter of the tile through LDS at a time, so three
+// workgroups share a CU and one's epilogue runs under the others' products (10k x 256 -> 688 with dg, du: 24.4 -> 20.5 us).
 template <int SP, int SQ>
-struct TileShape {
-  static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kPerCu = SP * SQ == 16 ? 1 : SQ == 1 ? 3 : 2;
+struct ProductShape {
+  static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kAtOnce = SQ > 2 ? 2 : SQ;
+  static constexpr int kPerCu = SP * SQ == 16 ? 1 : SQ == 1 ? 3 : 2;
+};
+template <int SP, int SQ>
+struct GateShape {
+  static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 ? 2 : 3;
 };
 
 struct GateArgs {
@@ -37,8 +45,8 @@ struct GateArgs {
 };
 
 template <typename T, int SP, int SQ>
-struct GateSides : TileShape<SP, SQ> {
-  using TileShape<SP, SQ>::kStep;
+struct GateSides : GateShape<SP, SQ> {
+  using GateShape<SP, SQ>::kStep;
   static constexpr int kHalf = SP * 32;      // units of a tile
   typedef Operand<T, kHalf, true, kStep> W;
   typedef Operand<T, SQ * 64, false, kStep> X;
@@ -61,7 +69,7 @@ struct GateSides : TileShape<SP, SQ> {
 };
 
 template <typename T, int SP, int SQ, bool BWD>
-__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
+__global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef GateSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -81,7 +89,7 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.c + S::W::kStepK - 1) / S::W::kStepK, acc);
 
   // a thread keeps four units for the whole epilogue
-  typedef TileRows<SP, SQ, S::kHalf> R;
+  typedef TileRows<SP, SQ, S::kHalf, S::kAtOnce> R;
   const int col = R::col(), f = f0 + col, n = a.f - f;
   float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
   if (a.bg) {
@@ -106,7 +114,7 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_kernel(
       for (int e = 0; e < 4; ++e) { sum[e] += o[e]; sum[4 + e] += v[e]; }
       put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
       put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
-      if (sizeof(T) == 2 && a.split) {
+      if (sizeof(T) == 2 && SQ < 4 && a.split) {      // problems this small take the smaller tiles
         f32x4 ro, rv;
 #pragma unroll
         for (int e = 0; e < 4; ++e) { ro[e] = o[e] - (float)(T)o[e]; rv[e] = v[e] - (float)(T)v[e]; }
@@ -208,8 +216,8 @@ struct GateDxArgs {
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
-struct DxSides : TileShape<SP, SQ> {
-  using TileShape<SP, SQ>::kStep;
+struct DxSides : ProductShape<SP, SQ> {
+  using ProductShape<SP, SQ>::kStep;
   typedef Operand<T, SP * 64, false, kStep> W;
   typedef Operand<T, SQ * 64, false, kStep> D;
   static constexpr int kStage = W::kBytes + D::kBytes, kLoads = W::kLoads + D::kLoads;
@@ -231,7 +239,7 @@ struct DxSides : TileShape<SP, SQ> {
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rd.get(s + W::kBytes, wq * SQ + j, ks); }
 };
 template <typename T, int SP, int SQ>
-__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dx_kernel(GateDxArgs a) {
+__global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_kernel(GateDxArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef DxSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -250,7 +258,7 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dx_kern
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, a.sides * s.half, acc);
-  typedef TileRows<SP, SQ, SP * 64> R;
+  typedef TileRows<SP, SQ, SP * 64, S::kAtOnce> R;
   const int wp = s.wp, c = c0 + R::col();
   auto pos = [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; };
   if (m0 + SQ * 64 <= a.rows && c0 + SP * 64 <= a.c && a.vec_out) {
@@ -279,8 +287,8 @@ struct GateDwArgs {
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
-struct DwSides : TileShape<SP, SQ> {
-  using TileShape<SP, SQ>::kStep;
+struct DwSides : ProductShape<SP, SQ> {
+  using ProductShape<SP, SQ>::kStep;
   typedef Operand<T, SP * 64, true, kStep> D;
   typedef Operand<T, SQ * 64, true, kStep> X;
   static constexpr int kStage = D::kBytes + X::kBytes, kLoads = D::kLoads + X::kLoads;
@@ -300,7 +308,7 @@ struct DwSides : TileShape<SP, SQ> {
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + D::kBytes, wq * SQ + j, ks); }
 };
 template <typename T, int SP, int SQ>
-__global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dw_kernel(GateDwArgs a) {
+__global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dw_kernel(GateDwArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef DwSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -320,7 +328,7 @@ __global__ __launch_bounds__(256, (TileShape<SP, SQ>::kPerCu)) void gate_dw_kern
   s.rx.init(lane);
   f32x16 acc[SP][SQ];
   tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.sides / 2) * s.once, acc);
-  typedef TileRows<SP, SQ, SP * 64> R;
+  typedef TileRows<SP, SQ, SP * 64, S::kAtOnce> R;
   const int wp = s.wp, p = p0 + R::col();
   float* const part = a.part + ((int64_t)strip * a.c + c0 + R::first()) * (2 * (int64_t)a.fp) + p;
   R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), s.wq, [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; }, [](int) {},
@@ -485,8 +493,8 @@ static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 //   gate, dW: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
 //   dx:       256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192, else as above
 enum Tile { kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
-static Tile tile_for(int64_t q, int64_t p, int64_t times = 1) {
-  if (ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
+static Tile tile_for(int64_t q, int64_t p, int64_t times = 1, bool wide = true) {
+  if (wide && ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
   return ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
 }
 static Tile tile_for_dx(int64_t rows, int64_t c) {
@@ -514,7 +522,7 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.ce = 16 / p.es;
   p.fp = (int)up_to(d->f, p.ce);
   p.cp = (int)up_to(d->c, p.ce);
-  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f);
+
   p.dx_tile = tile_for_dx(d->rows, d->c);
   p.pad_w = p.fp != d->f || d->param_dtype != d->dtype;
   p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
@@ -524,6 +532,8 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   // products that read them twice the arithmetic: nothing below 2^27 multiplications, where launches and latency decide (the backward
   // pass of 102 x 893 -> 391: 45 us either way), half as much time again above (16k x 512 -> 2048: 260 against 430 us).
   p.split = d->dtype == SSMI_BF16 && (double)d->rows * d->c * d->f <= (double)(1 << 27);
+  // float32 is bound by its matrix instructions: the wider tile's spared LDS reads buy nothing (16k x 256 -> 1024: 161 against 150 us)
+  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, 1, d->dtype == SSMI_BF16 && !p.split);
   p.dgu_bytes = up256((size_t)d->rows * (p.split ? 4 : 2) * p.fp * p.es);
   // strips of the weight gradient: one round of workgroups (two to a CU), each strip long enough to be worth its partial sums (512 rows)
   // and, in float32, short enough for the running sums (4096 rows: 2^-24 sqrt(4096) of a term)
@@ -594,21 +604,26 @@ static Staged stage_operands(const ssmi_gated_desc* d, const GatePlan& p, const 
   return s;
 }
 
-template <int SP, int SQ>
-static constexpr int tile_lds(int stages) { return stages > TileRows<SP, SQ, 64>::kBytes ? stages : TileRows<SP, SQ, 64>::kBytes; }
+template <typename S, int SP, int SQ>
+static constexpr int tile_lds() {
+  constexpr int stages = S::kStages * S::kStage, rows = TileRows<SP, SQ, 64, S::kAtOnce>::kBytes;
+  return stages > rows ? stages : rows;
+}
 
 template <typename T, int SP, int SQ, bool BWD>
 static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
   typedef GateSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
 template <typename T, bool BWD>
 static ssmi_status launch_gate(Tile t, const GateArgs& a, hipStream_t st) {
-  if (t == kTile128x256) return launch_gate_as<T, 2, 4, BWD>(a, st);
+  if constexpr (sizeof(T) == 2) {
+    if (t == kTile128x256) return launch_gate_as<T, 2, 4, BWD>(a, st);
+  }
   return t == kTile128x128 ? launch_gate_as<T, 2, 2, BWD>(a, st) : launch_gate_as<T, 2, 1, BWD>(a, st);
 }
 template <typename T, int SP, int SQ>
@@ -616,7 +631,7 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -625,7 +640,7 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   typedef DwSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
-  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<SP, SQ>(S::kStages * S::kStage)), st, a);
+  hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }

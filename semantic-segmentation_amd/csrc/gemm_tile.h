@@ -70,7 +70,7 @@ struct Operand {
   unsigned step_bytes;           // buffer offset from one K step to the next
 
   static __device__ __forceinline__ int swizzle(int row) {
-    if constexpr (!COLS) return STEP == 128 ? row & 7 : (row >> 2) & 3;
+    if constexpr (!COLS) return STEP == 128 ? (row >> 1) & 7 : (row >> 2) & 3;      // sixteen rows' 16-byte reads: all of the 64 banks
     if constexpr (sizeof(T) == 2) return kRowBytes >= 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
     return ((row >> 2) & 1) << 3;
   }
@@ -90,7 +90,7 @@ struct Operand {
         if (j == 0) k_in = rj;
       } else {
         voff[j] = rj < count ? (unsigned)(rj * ld * (int64_t)sizeof(T)) + piece * 16u : kOOB;
-        if (j == 0) k_in = piece * kElems;      // the same for every load: rows advance by multiples of eight
+        if (j == 0) k_in = piece * kElems;      // the same for every load: rows advance by multiples of sixteen
       }
     }
     step_bytes = COLS ? (unsigned)(ld * (kStepK * (int64_t)sizeof(T))) : (unsigned)STEP;
@@ -218,9 +218,9 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
 //   early(pass)                in front of a pass's LDS writes
 //   round(row, qc, i)          the lane's row of LDS values and its q: first() + qc.  UNROLL = kRounds makes qc and i constants, so that
 //                              an epilogue without branches keeps many rounds in flight and addresses its rows with scalars.
-template <int SP, int SQ, int COLS>
+template <int SP, int SQ, int COLS, int AT_ONCE = (SQ > 2 ? 2 : SQ)>
 struct TileRows {
-  static constexpr int kWidth = SP * 64, kStride = kWidth + 4, kAtOnce = SQ > 2 ? 2 : SQ, kRows = 64 * kAtOnce, kPasses = SQ / kAtOnce;
+  static constexpr int kWidth = SP * 64, kStride = kWidth + 4, kAtOnce = AT_ONCE, kRows = 64 * kAtOnce, kPasses = SQ / kAtOnce;
   static constexpr int kBytes = kRows * kStride * 4;
   static constexpr int kLanes = COLS / 4, kPerRound = 256 / kLanes, kRounds = kRows / kPerRound, kHalf = 32 * kAtOnce;
   static_assert(kHalf % kPerRound == 0 && COLS <= kWidth, "rounds stay inside a wave's rows");
@@ -249,7 +249,10 @@ struct TileRows {
           }
       __syncthreads();
 #pragma unroll UNROLL
-      for (int i = 0; i < kRounds; ++i) round(mine + i * kPerRound * kStride, q_of(pass, i), i);
+      for (int i = 0; i < kRounds; ++i) {
+        round(mine + i * kPerRound * kStride, q_of(pass, i), i);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // four rounds in flight: more cost registers the accumulators need
+      }
     }
   }
 };
