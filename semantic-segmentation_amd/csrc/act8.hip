@@ -8,71 +8,103 @@
 // bfloat16 and float32 (four significant bits times a power of two).  Scales under 2^-111 are not used: every intermediate
 // stays a normal float32.  A group that holds an infinity or a NaN restores as NaN.
 //
-// The passes move bytes and nothing else binds them: four lanes share a group, a lane owns eight channels (16 bytes of
-// bfloat16 in, 8 bytes of codes out), the group's maximum is two cross-lane steps on the integer patterns of |x| (which order as
-// the values do and put infinities and NaN on top).
+// The passes move bytes and nothing else binds them: a lane owns 16 bytes of a pixel (eight bfloat16 or four float32 channels, so that a
+// wave's accesses are whole lines), four or eight lanes share a group, and the group's maximum is two or three cross-lane steps on the
+// integer patterns of |x| (which order as the values do and put infinities and NaN on top).
+// Measured: store + restore of 1M x 64 bfloat16 pixels 40 us, 5.2 TB/s of the 407 MB that they move (a large copy: 5.2 TB/s).
 #include "common.h"
 
 namespace ssmi {
 
 static constexpr int kGroup = 32;
 
-// rows of 8 channels as they travel; VEC: the lane's channels are all there or all absent and 16-byte accesses are allowed
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+template <typename T> struct Piece {
+  static constexpr int kCh = 16 / (int)sizeof(T), kLanes = kGroup / kCh, kAtOnce = 256 / kLanes;      // channels a lane, lanes a group, groups a block
+};
+
+// a lane's channels as they travel; VEC: all there or all absent, and 16-byte accesses are allowed
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void load_piece(const T* p, int n, float (&v)[N]) {
   if constexpr (VEC) {
-    const f32x4 a = Act<T>::gld4(p), b = Act<T>::gld4(p + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-  } else {
+    for (int q = 0; q < N; q += 4) {
+      const f32x4 a = Act<T>::gld4(p + q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? Act<T>::gld(p + i) : 0.f;
-  }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-  if constexpr (VEC) {
-    const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    if constexpr (sizeof(T) == 2) {
-      const u32x2 x = pack_bf16x4(a), y = pack_bf16x4(b);
-      *reinterpret_cast<u32x4*>(p) = u32x4{x[0], x[1], y[0], y[1]};
-    } else {
-      Act<T>::gst4(p, a);
-      Act<T>::gst4(p + 4, b);
+      for (int i = 0; i < 4; ++i) v[q + i] = a[i];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i) v[i] = i < n ? Act<T>::gld(p + i) : 0.f;
+  }
+}
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void store_piece(T* p, int n, const float (&v)[N]) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      const u32x2 x = pack_bf16x4(f32x4{v[0], v[1], v[2], v[3]}), y = pack_bf16x4(f32x4{v[4], v[5], v[6], v[7]});
+      *reinterpret_cast<u32x4*>(p) = u32x4{x[0], x[1], y[0], y[1]};
+    } else {
+      Act<T>::gst4(p, f32x4{v[0], v[1], v[2], v[3]});
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
       if (i < n) Act<T>::gst(p + i, v[i]);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ u32x2 load_codes(const uint8_t* p, int n) {
-  if constexpr (VEC) return *reinterpret_cast<const u32x2*>(p);
-  u32x2 w = {0u, 0u};
+// N codes, four to a word
+template <bool VEC, int N>
+__device__ __forceinline__ void load_codes(const uint8_t* p, int n, unsigned (&w)[N / 4]) {
+  if constexpr (VEC && N == 8) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    w[0] = v[0];
+    w[1] = v[1];
+  } else if constexpr (VEC) {
+    w[0] = *reinterpret_cast<const unsigned*>(p);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) w[i >> 2] |= (unsigned)p[i] << (8 * (i & 3));
-  return w;
+    for (int k = 0; k < N / 4; ++k) w[k] = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) w[i >> 2] |= (unsigned)p[i] << (8 * (i & 3));
+  }
+}
+template <bool VEC, int N>
+__device__ __forceinline__ void store_codes(uint8_t* p, int n, const unsigned (&w)[N / 4]) {
+  if constexpr (VEC && N == 8) {
+    *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+  } else if constexpr (VEC) {
+    *reinterpret_cast<unsigned*>(p) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+  }
 }
 
-// How a block's 64 lane quartets lie over the tensor: `gp` groups of a pixel side by side (all of them up to 64, then
+// How a block's lane groups lie over the tensor: `gp` groups of a pixel side by side (all of them up to a block's worth, then
 // blockIdx.y counts further), `ppb` pixels at a time.  A lane keeps its channels for the whole kernel, so the parameters of its
 // BatchNormalization are loaded once, and walks pixels in steps of the grid.
 struct Lane {
   int64_t pix, step;      // first pixel, pixels from one step to the next
   int g, ch, n;           // group, first channel, channels (<= 0: none)
+  bool lead;              // the first lane of its group
 };
+template <typename T>
+__device__ __forceinline__ int pixels_at_once(int groups) { return Piece<T>::kAtOnce / min(groups, Piece<T>::kAtOnce); }
+template <typename T>
 __device__ __forceinline__ Lane lane_of(int c, int groups) {
-  const int gp = min(groups, 64), ppb = 64 / gp;
-  const int lg = threadIdx.x >> 2, part = threadIdx.x & 3;
+  typedef Piece<T> P;
+  const int gp = min(groups, P::kAtOnce), ppb = P::kAtOnce / gp;
+  const int lg = (int)threadIdx.x / P::kLanes, part = (int)threadIdx.x % P::kLanes;
   const int p = lg / gp;
   Lane l;
-  l.g = lg - p * gp + 64 * (int)blockIdx.y;
+  l.g = lg - p * gp + P::kAtOnce * (int)blockIdx.y;
   l.pix = (int64_t)blockIdx.x * ppb + p;
   l.step = (int64_t)gridDim.x * ppb;
-  l.ch = l.g * kGroup + part * 8;
-  l.n = p < ppb && l.g < groups ? min(8, c - l.ch) : 0;
+  l.ch = l.g * kGroup + part * P::kCh;
+  l.n = p < ppb && l.g < groups ? min(P::kCh, c - l.ch) : 0;
+  l.lead = part == 0;
   return l;
 }
 
@@ -81,46 +113,39 @@ static constexpr int kSteps = 4;      // pixels per lane and round: independent 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void act8_store_kernel(const T* __restrict__ x, int64_t ld, int64_t npix, int c, int groups,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const Lane l = lane_of(c, groups);
+  typedef Piece<T> P;
+  constexpr int N = P::kCh;
+  const Lane l = lane_of<T>(c, groups);
   // a block's lanes stay together (the maximum crosses lanes): rounds go by its first pixel
-  for (int64_t base = (int64_t)blockIdx.x * (64 / min(groups, 64)), pix = l.pix; base < npix; base += kSteps * l.step, pix += kSteps * l.step) {
-    float v[kSteps][8];
+  for (int64_t base = (int64_t)blockIdx.x * pixels_at_once<T>(groups), pix = l.pix; base < npix; base += kSteps * l.step, pix += kSteps * l.step) {
+    float v[kSteps][N];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
-      if (l.n > 0 && pix + s * l.step < npix) load8<T, VEC>(x + (pix + s * l.step) * ld + l.ch, l.n, v[s]);
+      for (int i = 0; i < N; ++i) v[s][i] = 0.f;
+      if (l.n > 0 && pix + s * l.step < npix) load_piece<T, VEC>(x + (pix + s * l.step) * ld + l.ch, l.n, v[s]);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       unsigned top = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(unsigned, v[s][i]) & 0x7FFFFFFFu);
-      top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
-      top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
+      for (int i = 0; i < N; ++i) top = max(top, __builtin_bit_cast(unsigned, v[s][i]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = 1; o < P::kLanes; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
       const bool fine = top < 0x7F800000u;
       // 464 / 256 = 1.8125: a mantissa above it carries into the exponent
       const int e = max((int)((top + 0x17FFFFu) >> 23) - 8, 16);
       const float inv = __builtin_bit_cast(float, (unsigned)(254 - (fine ? e : 127)) << 23);
-      u32x2 w = {0u, 0u};
-      if (fine) {
+      unsigned w[N / 4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k] * inv, v[s][4 * k + 1] * inv, 0, false);
-          w[k] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k + 2] * inv, v[s][4 * k + 3] * inv, q, true);
-        }
+      for (int k = 0; k < N / 4; ++k) {
+        const int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k] * inv, v[s][4 * k + 1] * inv, 0, false);
+        w[k] = fine ? (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k + 2] * inv, v[s][4 * k + 3] * inv, q, true) : 0u;
       }
       const int64_t px = pix + s * l.step;
       if (l.n > 0 && px < npix) {
-        uint8_t* const d = codes + px * c + l.ch;
-        if constexpr (VEC) {
-          *reinterpret_cast<u32x2*>(d) = w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < l.n) d[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-        }
-        if ((threadIdx.x & 3) == 0) scales[px * groups + l.g] = (uint8_t)(fine ? e : 255);
+        store_codes<VEC, N>(codes + px * c + l.ch, l.n, w);
+        if (l.lead) scales[px * groups + l.g] = (uint8_t)(fine ? e : 255);
       }
     }
   }
@@ -133,11 +158,12 @@ struct RestoreBn {
   int64_t hw;
 };
 
-__device__ __forceinline__ void decode8(u32x2 w, unsigned byte, float (&v)[8]) {
+template <int N>
+__device__ __forceinline__ void decode(const unsigned (&w)[N / 4], unsigned byte, float (&v)[N]) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const float s = __builtin_bit_cast(float, byte == 255u ? 0x7FC00000u : byte << 23);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < N / 4; ++k) {
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
     v[4 * k] = a[0] * s;
     v[4 * k + 1] = a[1] * s;
@@ -152,12 +178,13 @@ template <typename T, bool VEC, bool BN>
 __global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t npix, int c,
                                                            int groups, T* __restrict__ y, int64_t ld_y, RestoreBn bn, T* __restrict__ out,
                                                            int64_t ld_out) {
-  const Lane l = lane_of(c, groups);
+  constexpr int N = Piece<T>::kCh;
+  const Lane l = lane_of<T>(c, groups);
   if (l.n <= 0) return;
-  float mean[8], invstd[8], gamma[8], beta[8], slope[8];
+  float mean[N], invstd[N], gamma[N], beta[N], slope[N];
   if constexpr (BN) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int k = min(l.ch + i, c - 1);
       mean[i] = bn.mean[k];
       invstd[i] = bn.invstd[k];
@@ -167,39 +194,35 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __rest
     }
   }
   for (int64_t pix = l.pix; pix < npix; pix += kSteps * l.step) {
-    u32x2 w[kSteps];
-    unsigned sc[kSteps];
+    unsigned w[kSteps][N / 4], sc[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      w[s] = u32x2{0u, 0u};
-      sc[s] = 127;
-      if (pix + s * l.step < npix) {
-        w[s] = load_codes<VEC>(codes + (pix + s * l.step) * c + l.ch, l.n);
-        sc[s] = scales[(pix + s * l.step) * groups + l.g];
-      }
+      const int64_t px = min(pix + s * l.step, npix - 1);      // past the end: the last pixel again, not stored
+      load_codes<VEC, N>(codes + px * c + l.ch, l.n, w[s]);
+      sc[s] = scales[px * groups + l.g];
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int64_t px = pix + s * l.step;
       if (px >= npix) break;
-      float v[8];
-      decode8(w[s], sc[s], v);
-      if (!BN || y) store8<T, VEC>(y + px * ld_y + l.ch, l.n, v);
+      float v[N];
+      decode<N>(w[s], sc[s], v);
+      if (!BN || y) store_piece<T, VEC>(y + px * ld_y + l.ch, l.n, v);
       if constexpr (BN) {
-        float drop[8];
+        float drop[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) drop[i] = 1.f;
+        for (int i = 0; i < N; ++i) drop[i] = 1.f;
         if (bn.drop) {
           const int64_t img = npix <= 0xFFFFFFFFll ? (int64_t)((unsigned)px / (unsigned)bn.hw) : px / bn.hw;      // hw <= npix
-          load8<float, VEC>(bn.drop + img * c + l.ch, l.n, drop);
+          load_piece<float, VEC>(bn.drop + img * c + l.ch, l.n, drop);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
           const float z = gamma[i] * ((v[i] - mean[i]) * invstd[i]) + beta[i];      // the order of bn_act_fwd_kernel
           const float r = z > 0.f ? z : slope[i] * z;
           v[i] = r * drop[i];
         }
-        store8<T, VEC>(out + px * ld_out + l.ch, l.n, v);
+        store_piece<T, VEC>(out + px * ld_out + l.ch, l.n, v);
       }
     }
   }
@@ -212,9 +235,11 @@ static ssmi_status check_sizes(const char* who, int64_t npix, int32_t c) {
   return SSMI_OK;
 }
 // sixteen rounds of four pixels a lane at the most (the parameters are loaded once per lane), but enough blocks to fill the card
+template <typename T>
 static inline dim3 blocks_for(int64_t npix, int groups) {
-  const int gp = groups < 64 ? groups : 64, ny = (groups + 63) / 64;
-  const int64_t all = ceil_div64(npix, (int64_t)(64 / gp) * kSteps);
+  constexpr int at_once = Piece<T>::kAtOnce;
+  const int gp = groups < at_once ? groups : at_once, ny = (groups + at_once - 1) / at_once;
+  const int64_t all = ceil_div64(npix, (int64_t)(at_once / gp) * kSteps);
   int64_t nx = ceil_div64(all, 16);
   const int64_t fill = ceil_div64(4096, ny);
   if (nx < fill) nx = all < fill ? all : fill;
@@ -238,8 +263,8 @@ ssmi_status ssmi_act8_store(const void* x, int64_t ld, int64_t npix, int32_t c, 
     using T = decltype(tag);
     const bool vec = c % 8 == 0 && ld % 8 == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     const T* xt = static_cast<const T*>(x);
-    if (vec) hipLaunchKernelGGL((act8_store_kernel<T, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
-    else hipLaunchKernelGGL((act8_store_kernel<T, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
+    if (vec) hipLaunchKernelGGL((act8_store_kernel<T, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
+    else hipLaunchKernelGGL((act8_store_kernel<T, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), xt, ld, npix, c, groups, codes, scales);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
@@ -256,8 +281,8 @@ ssmi_status ssmi_act8_restore(const uint8_t* codes, const uint8_t* scales, int64
     const bool vec = c % 8 == 0 && ld_y % 8 == 0 && aligned16(y) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     T* yt = static_cast<T*>(y);
     const RestoreBn none = {};
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
@@ -280,8 +305,8 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
     using T = decltype(tag);
     const bool vec = c % 8 == 0 && ld_out % 8 == 0 && aligned16(out) && (!y || (ld_y % 8 == 0 && aligned16(y))) && (!drop || aligned16(drop)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     T *yt = static_cast<T*>(y), *ot = static_cast<T*>(out);
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true>), blocks_for(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
