@@ -56,11 +56,11 @@ struct GateSides : GateShape<SP, SQ> {
   typename W::Reader rw;
   typename X::Reader rx;
   int c, wp, wq;
-  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+  __device__ __forceinline__ void one(lds_bytes s, int t, int j) const {
     const int left = c - t * W::kStepK;
-    wg.request(s, t, left);
-    wu.request(s + W::kBytes, t, left);
-    x.request(s + 2 * W::kBytes, t, left);
+    if (j < W::kLoads) wg.one(s, t, j, left);
+    else if (j < 2 * W::kLoads) wu.one(s + W::kBytes, t, j - W::kLoads, left);
+    else x.one(s + 2 * W::kBytes, t, j - 2 * W::kLoads, left);
   }
   __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const {
     return rw.get(s + (i / (SP / 2)) * W::kBytes, wp * (SP / 2) + i % (SP / 2), ks);
@@ -226,14 +226,17 @@ struct DxSides : ProductShape<SP, SQ> {
   __amdgpu_buffer_rsrc_t wu;
   typename W::Reader rw;
   typename D::Reader rd;
-  int fp, half, wp, wq;
-  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+  int fp, half, sides, wp, wq;
+  __device__ __forceinline__ void one(lds_bytes s, int t, int j) const {
     const int side = t >= 2 * half ? (t >= 3 * half ? 3 : 2) : t >= half ? 1 : 0;
-    const int ts = t - side * half, left = fp - ts * W::kStepK;
-    W w = wg;
-    if (side & 1) w.rsrc = wu;
-    w.request(s, ts, left);
-    d.request(s + W::kBytes, ts, left, (unsigned)(side * fp * (int)sizeof(T)));
+    const int ts = t - side * half, left = t < sides * half ? fp - ts * W::kStepK : 0;
+    if (j < W::kLoads) {
+      W w = wg;
+      if (side & 1) w.rsrc = wu;
+      w.one(s, ts, j, left);
+    } else {
+      d.one(s + W::kBytes, ts, j - W::kLoads, left, (unsigned)(side * fp * (int)sizeof(T)));
+    }
   }
   __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rw.get(s, wp * SP + i, ks); }
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rd.get(s + W::kBytes, wq * SQ + j, ks); }
@@ -248,6 +251,7 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_k
   const int c0 = at.p * (SP * 64);
   S s;
   s.fp = a.fp;
+  s.sides = a.sides;
   s.half = (a.fp + S::W::kStepK - 1) / S::W::kStepK;
   s.wp = wave >> 1;
   s.wq = wave & 1;
@@ -296,13 +300,13 @@ struct DwSides : ProductShape<SP, SQ> {
   X x;
   typename D::Reader rd;
   typename X::Reader rx;
-  int rows, once, wp, wq;
+  int rows, once, times, wp, wq;
   unsigned second;      // bytes from the first terms of a row to the second ones
-  __device__ __forceinline__ void request(lds_bytes s, int t) const {
+  __device__ __forceinline__ void one(lds_bytes s, int t, int j) const {
     const bool again = t >= once;
-    const int ts = again ? t - once : t, left = rows - ts * D::kStepK;
-    d.request(s, ts, left, again ? second : 0u);
-    x.request(s + D::kBytes, ts, left);
+    const int ts = again ? t - once : t, left = t < times * once ? rows - ts * D::kStepK : 0;
+    if (j < D::kLoads) d.one(s, ts, j, left, again ? second : 0u);
+    else x.one(s + D::kBytes, ts, j - D::kLoads, left);
   }
   __device__ __forceinline__ u32x4 p(lds_bytes s, int i, int ks) const { return rd.get(s, wp * SP + i, ks); }
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + D::kBytes, wq * SQ + j, ks); }
@@ -322,12 +326,13 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dw_k
   s.wq = wave & 1;
   s.d.init(static_cast<const T*>(a.dgu) + m0 * (a.sides * (int64_t)a.fp) + p0, a.sides * (int64_t)a.fp, 2 * a.fp - p0);
   s.once = (s.rows + S::D::kStepK - 1) / S::D::kStepK;
+  s.times = a.sides / 2;
   s.second = 2u * (unsigned)a.fp * (unsigned)sizeof(T);
   s.x.init(static_cast<const T*>(a.x) + m0 * a.x_ld + c0, a.x_ld, a.cp - c0);
   s.rd.init(lane);
   s.rx.init(lane);
   f32x16 acc[SP][SQ];
-  tile_product<T, SP, SQ>(s, (lds_bytes)smem, (a.sides / 2) * s.once, acc);
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, s.times * s.once, acc);
   typedef TileRows<SP, SQ, SP * 64, S::kAtOnce> R;
   const int wp = s.wp, p = p0 + R::col();
   float* const part = a.part + ((int64_t)strip * a.c + c0 + R::first()) * (2 * (int64_t)a.fp) + p;

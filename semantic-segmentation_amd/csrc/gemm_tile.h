@@ -96,17 +96,11 @@ struct Operand {
     step_bytes = COLS ? (unsigned)(ld * (kStepK * (int64_t)sizeof(T))) : (unsigned)STEP;
   }
 
-  // requests K step t into the stage at `lds`; left: valid k from this step's first on; skip: bytes in front of step 0
-  __device__ __forceinline__ void request(lds_bytes lds, int t, int left, unsigned skip = 0) const {
-    const unsigned soff = (unsigned)t * step_bytes + skip;
-    const unsigned dst = (unsigned)(uintptr_t)lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-    if (left >= kStepK) {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) stage16(rsrc, voff[j], soff, dst + j * 4096);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) stage16(rsrc, (COLS ? k_in + j * kRowsPerLoad : k_in) < left ? voff[j] : kOOB, soff, dst + j * 4096);
-    }
+  // load j of K step t into the stage at `lds`; left: valid k from this step's first on (<= 0: none, zeros arrive); skip: bytes in
+  // front of step 0
+  __device__ __forceinline__ void one(lds_bytes lds, int t, int j, int left, unsigned skip = 0) const {
+    stage16(rsrc, (COLS ? k_in + j * kRowsPerLoad : k_in) < left ? voff[j] : kOOB, (unsigned)t * step_bytes + skip,
+            (unsigned)(uintptr_t)lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + j * 4096);
   }
 
   // the lane's part of fragment (32 indices from 32 * s on, k piece ks of four): eight bfloat16 or four float32
@@ -159,9 +153,11 @@ __device__ __forceinline__ f32x16 mfma_step(u32x4 p, u32x4 q, f32x16 c) {
   }
 }
 
-// The K loop of a tile.  Sides: request(stage, t) stages step t, p(stage, i, ks) / q(stage, j, ks) read fragments.  Fragments are read
-// one k piece ahead of their arithmetic, also over the step boundary: the barrier sits in front of a step's LAST piece, whose
-// fragments are in registers already, so the first reads of the next step run under it.
+// The K loop of a tile.  Sides: one(stage, t, j) is load j of step t (zeros for a step past the last), p(stage, i, ks) / q(stage, j, ks)
+// read fragments.  Fragments are read one k piece ahead of their arithmetic, also over the step boundary: the barrier sits in front of a
+// step's LAST piece, whose fragments are in registers already.  Behind it the next step's first reads and the loads of step t + kStages
+// go between that piece's matrix instructions, one load each: in a row they would leave the matrix unit idle for as long as they take
+// to issue.  Every step issues the same loads, so the waits count them and the loop has no special ends.
 template <typename T, int SP, int SQ, typename Sides>
 __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, int steps, f32x16 (&acc)[SP][SQ]) {
 #pragma unroll
@@ -170,8 +166,7 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
     for (int j = 0; j < SQ; ++j)
 #pragma unroll
       for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
-  if (steps <= 0) return;
-  constexpr int kStage = Sides::kStage;
+    constexpr int kStage = Sides::kStage;
   u32x4 p[2][SP], q[2][SQ];
   auto read = [&](int buf, lds_bytes stage, int ks) {
 #pragma unroll
@@ -186,9 +181,12 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
       for (int j = 0; j < SQ; ++j) acc[i][j] = mfma_step<T>(p[buf][i], q[buf][j], acc[i][j]);
   };
   constexpr int kStages = Sides::kStages, kPieces = Sides::kStep / 32, kAhead = (kStages - 2) * Sides::kLoads;
-  for (int t = 0; t < kStages && t < steps; ++t) sides.request(lds + t * kStage, t);
-  if (steps >= kStages) stage_wait<(kStages - 1) * Sides::kLoads>();
-  else stage_wait<0>();
+  constexpr int kLoads = Sides::kLoads, kPer = (kLoads + SP * SQ - 1) / (SP * SQ);
+#pragma unroll
+  for (int t = 0; t < kStages; ++t)
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) sides.one(lds + t * kStage, t, j);
+  stage_wait<(kStages - 1) * kLoads>();
   __syncthreads();
   read(0, lds, 0);
   int at = 0;
@@ -201,14 +199,20 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
       read((ks + 1) & 1, cur, ks + 1);
       multiply(ks & 1);
     }
-    if (t + kStages <= steps) stage_wait<kAhead>();      // all of steps t + 1 .. t + kStages - 1 were requested: the first is there
-    else stage_wait<0>();
+    stage_wait<kAhead>();
     __syncthreads();      // step t + 1 is there for everyone, and nobody reads step t any more
     __builtin_amdgcn_sched_barrier(0);
-    if (t + kStages < steps) sides.request(cur, t + kStages);
-    if (t + 1 < steps) read(0, nxt, 0);
-    multiply(1);
+    read(0, nxt, 0);
+#pragma unroll
+    for (int m = 0; m < SP * SQ; ++m) {
+      acc[m / SQ][m % SQ] = mfma_step<T>(p[1][m / SQ], q[1][m % SQ], acc[m / SQ][m % SQ]);
+#pragma unroll
+      for (int j = m * kPer; j < (m + 1) * kPer && j < kLoads; ++j) sides.one(cur, t + kStages, j);
+      if (m * kPer < kLoads) __builtin_amdgcn_sched_barrier(0);
+    }
   }
+  stage_wait<0>();      // the zeros of the steps past the last: the epilogue takes the LDS over
+  __syncthreads();
 }
 
 // The accumulators of a tile as rows in LDS, for an epilogue in memory order: q rows of 2 * 32 * SP float32 values; consecutive lanes
