@@ -26,9 +26,9 @@ struct ProductShape {
   static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kAtOnce = SQ > 2 ? 2 : SQ;
   static constexpr int kPerCu = SP * SQ == 16 ? 1 : SQ == 1 ? 3 : 2;
 };
-template <int SP, int SQ>
+template <typename T, int SP, int SQ>
 struct GateShape {
-  static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 ? 2 : 3;
+  static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 || (SQ == 2 && sizeof(T) == 4) ? 2 : 3;
 };
 
 struct GateArgs {
@@ -45,8 +45,8 @@ struct GateArgs {
 };
 
 template <typename T, int SP, int SQ>
-struct GateSides : GateShape<SP, SQ> {
-  using GateShape<SP, SQ>::kStep;
+struct GateSides : GateShape<T, SP, SQ> {
+  using GateShape<T, SP, SQ>::kStep;
   static constexpr int kHalf = SP * 32;      // units of a tile
   typedef Operand<T, kHalf, true, kStep> W;
   typedef Operand<T, SQ * 64, false, kStep> X;
@@ -69,7 +69,7 @@ struct GateSides : GateShape<SP, SQ> {
 };
 
 template <typename T, int SP, int SQ, bool BWD>
-__global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
+__global__ __launch_bounds__(256, (GateShape<T, SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef GateSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -497,15 +497,20 @@ static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 // Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
 //   gate, dW: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
 //   dx:       256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192, else as above
+// float32 stays with the last two: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
 enum Tile { kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
-static Tile tile_for(int64_t q, int64_t p, int64_t times = 1, bool wide = true) {
+static Tile tile_for(int64_t q, int64_t p, bool wide, int64_t times = 1) {
   if (wide && ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
   return ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
 }
-static Tile tile_for_dx(int64_t rows, int64_t c) {
-  if (c > 128 && ceil_div64(rows, 256) * ceil_div64(c, 256) >= 192) return kTile256x256;
-  const Tile t = tile_for(rows, c);
-  return t == kTile128x256 ? kTile128x128 : t;
+static Tile tile_for_dx(int64_t rows, int64_t c, bool wide) {
+  if (wide && c > 128 && ceil_div64(rows, 256) * ceil_div64(c, 256) >= 192) return kTile256x256;
+  return tile_for(rows, c, false);
+}
+static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t most_strips) {
+  // the larger tile only under strips of 4096 rows, where its own speed outweighs the partial sums of twice the strips
+  if (wide && c > 128 && rows / ceil_div64(512, ceil_div64(p, 128) * ceil_div64(c, 256)) >= 4096) return kTile128x256;
+  return tile_for(c, p, false, most_strips);
 }
 static inline int64_t q_side(Tile t) { return t == kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
 
@@ -528,7 +533,8 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.fp = (int)up_to(d->f, p.ce);
   p.cp = (int)up_to(d->c, p.ce);
 
-  p.dx_tile = tile_for_dx(d->rows, d->c);
+  const bool bf = d->dtype == SSMI_BF16;
+  p.dx_tile = tile_for_dx(d->rows, d->c, bf);
   p.pad_w = p.fp != d->f || d->param_dtype != d->dtype;
   p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
   p.w_bytes = p.pad_w ? 2 * up256((size_t)d->c * p.fp * p.es) : 0;
@@ -536,17 +542,13 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   // One bfloat16 of dg and du is off by 2^-9 on average and shows beside the output's own rounding; two are exact to 2^-17 and cost the two
   // products that read them twice the arithmetic: nothing below 2^27 multiplications, where launches and latency decide (the backward
   // pass of 102 x 893 -> 391: 45 us either way), half as much time again above (16k x 512 -> 2048: 260 against 430 us).
-  p.split = d->dtype == SSMI_BF16 && (double)d->rows * d->c * d->f <= (double)(1 << 27);
-  // float32 is bound by its matrix instructions: the wider tile's spared LDS reads buy nothing (16k x 256 -> 1024: 161 against 150 us)
-  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, 1, d->dtype == SSMI_BF16 && !p.split);
+  p.split = bf && (double)d->rows * d->c * d->f <= (double)(1 << 27);
+  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, bf && !p.split);      // the wide tile's epilogue has no registers for the second terms
   p.dgu_bytes = up256((size_t)d->rows * (p.split ? 4 : 2) * p.fp * p.es);
   // strips of the weight gradient: one round of workgroups (two to a CU), each strip long enough to be worth its partial sums (512 rows)
   // and, in float32, short enough for the running sums (4096 rows: 2^-24 sqrt(4096) of a term)
-  const int64_t most = ceil_div64(d->rows, 512), least = d->dtype == SSMI_BF16 ? 1 : ceil_div64(d->rows, 4096);
-  // and the larger tile only under strips of 4096 rows, where its own speed outweighs the partial sums of twice the strips
-  const int64_t wide = ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, 256);
-  p.dw_tile = d->c > 128 && d->rows / ceil_div64(512, wide) >= 4096 ? kTile128x256 : tile_for(d->c, 2 * p.fp, most);
-  if (p.dw_tile == kTile128x256 && d->rows / ceil_div64(512, wide) < 4096) p.dw_tile = kTile128x128;
+  const int64_t most = ceil_div64(d->rows, 512), least = bf ? 1 : ceil_div64(d->rows, 4096);
+  p.dw_tile = tile_for_dw(d->rows, d->c, 2 * p.fp, bf, most);
   int64_t strips = ceil_div64(512, ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, q_side(p.dw_tile)));
   strips = strips < most ? strips : most;
   strips = strips > least ? strips : least;
@@ -650,6 +652,21 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   return SSMI_OK;
 }
 
+template <typename T>
+static ssmi_status launch_dx(Tile t, const GateDxArgs& a, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (t == kTile256x256) return launch_dx_as<T, 4, 4>(a, st);
+  }
+  return t == kTile128x128 ? launch_dx_as<T, 2, 2>(a, st) : launch_dx_as<T, 2, 1>(a, st);
+}
+template <typename T>
+static ssmi_status launch_dw(Tile t, const GateDwArgs& a, int strips, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (t == kTile128x256) return launch_dw_as<T, 2, 4>(a, strips, st);
+  }
+  return t == kTile128x128 ? launch_dw_as<T, 2, 2>(a, strips, st) : launch_dw_as<T, 2, 1>(a, strips, st);
+}
+
 template <typename T, typename P, int MB>
 static void launch_rows_mb(const GateArgs& a, bool vec, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div64(a.f, 32), (unsigned)ceil_div64(a.rows, MB));
@@ -713,14 +730,14 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
     GateDxArgs b = {};
     b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp; b.sides = sides;
     b.vec_out = d->x_ld % 4 == 0 && aligned(dx, 4 * p.es);
-    r = p.dx_tile == kTile256x256 ? launch_dx_as<T, 4, 4>(b, st) : p.dx_tile == kTile128x128 ? launch_dx_as<T, 2, 2>(b, st) : launch_dx_as<T, 2, 1>(b, st);
+    r = launch_dx<T>(p.dx_tile, b, st);
     if (r != SSMI_OK) return r;
   }
   const bool dw = dwg || dwu;
   if (dw) {
     GateDwArgs b = {};
     b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp; b.sides = sides;
-    r = p.dw_tile == kTile128x256 ? launch_dw_as<T, 2, 4>(b, p.strips, st) : p.dw_tile == kTile128x128 ? launch_dw_as<T, 2, 2>(b, p.strips, st) : launch_dw_as<T, 2, 1>(b, p.strips, st);
+    r = launch_dw<T>(p.dw_tile, b, p.strips, st);
     if (r != SSMI_OK) return r;
   }
   if (dw || a.db) {
