@@ -25,10 +25,12 @@ template <int SP, int SQ>
 struct ProductShape {
   static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kAtOnce = SQ > 2 ? 2 : SQ;
   static constexpr int kPerCu = SP * SQ == 16 ? 1 : SQ == 1 ? 3 : 2;
+  static constexpr bool kChunks = true;
 };
-template <typename T, int SP, int SQ>
+template <int SP, int SQ>
 struct GateShape {
-  static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 || (SQ == 2 && sizeof(T) == 4) ? 2 : 3;
+  static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 ? 2 : 3;
+  static constexpr bool kChunks = false;      // K = channels: a running sum is as exact as the plain form's
 };
 
 struct GateArgs {
@@ -45,8 +47,8 @@ struct GateArgs {
 };
 
 template <typename T, int SP, int SQ>
-struct GateSides : GateShape<T, SP, SQ> {
-  using GateShape<T, SP, SQ>::kStep;
+struct GateSides : GateShape<SP, SQ> {
+  using GateShape<SP, SQ>::kStep;
   static constexpr int kHalf = SP * 32;      // units of a tile
   typedef Operand<T, kHalf, true, kStep> W;
   typedef Operand<T, SQ * 64, false, kStep> X;
@@ -69,7 +71,7 @@ struct GateSides : GateShape<T, SP, SQ> {
 };
 
 template <typename T, int SP, int SQ, bool BWD>
-__global__ __launch_bounds__(256, (GateShape<T, SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
+__global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef GateSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

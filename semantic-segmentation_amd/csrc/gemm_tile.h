@@ -158,7 +158,7 @@ __device__ __forceinline__ f32x16 mfma_step(u32x4 p, u32x4 q, f32x16 c) {
 // step's LAST piece, whose fragments are in registers already.  Behind it the next step's first reads and the loads of step t + kStages
 // go between that piece's matrix instructions, one load each: in a row they would leave the matrix unit idle for as long as they take
 // to issue.  Every step issues the same loads, so the waits count them and the loop has no special ends.
-// float32 sums go in chunks of 256 k that are added up at their ends: the error of a running sum grows with the root of its length, and
+// float32 sums over long axes (Sides::kChunks) go in chunks of 256 k that are added up at their ends: the error of a running sum grows with the root of its length, and
 // one chunk's plus one sum over chunks stays under that of the plain form's library products (without: 8e-7 at 1440 k, theirs 3e-7).
 template <typename T, int SP, int SQ, typename Sides>
 __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, int steps, f32x16 (&acc)[SP][SQ]) {
@@ -191,7 +191,7 @@ __device__ __forceinline__ void tile_product(const Sides& sides, lds_bytes lds, 
   stage_wait<(kStages - 1) * kLoads>();
   __syncthreads();
   read(0, lds, 0);
-  constexpr bool kChunks = sizeof(T) == 4;
+  constexpr bool kChunks = sizeof(T) == 4 && Sides::kChunks;
   constexpr int kChunkSteps = 256 * (int)sizeof(T) / Sides::kStep;
   f32x16 sum[kChunks ? SP : 1][kChunks ? SQ : 1];
   if constexpr (kChunks) {
