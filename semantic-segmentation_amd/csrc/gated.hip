@@ -8,6 +8,8 @@
 // then  dx = dg Wg^T + du Wu^T  (one product over 2 f) and  dW = x^T dg, x^T du  (one product over the rows, split into strips whose
 // float32 partial sums are added in a fixed order: results do not depend on the launch).
 // All products run on gemm_tile.h: bfloat16 32x32x16 or float32 32x32x2 matrix instructions, float32 sums throughout.
+#include <algorithm>
+
 #include "gate_act.h"
 #include "gemm_tile.h"
 
@@ -554,7 +556,10 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   int64_t strips = ceil_div64(512, ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, q_side(p.dw_tile)));
   strips = strips < most ? strips : most;
   strips = strips > least ? strips : least;
-  p.strip_rows = up_to(ceil_div64(d->rows, strips), 64);
+  // a strip is addressed with 32-bit offsets from its first row: under 2^31 - 2^27 bytes of [dg | du] and of x
+  const int64_t row_bytes = p.es * std::max<int64_t>((p.split ? 4 : 2) * (int64_t)p.fp, p.pad_x ? p.cp : d->x_ld);
+  const int64_t reach = std::max<int64_t>(((1ll << 31) - (1ll << 27)) / row_bytes / 64 * 64, 64);
+  p.strip_rows = std::min(up_to(ceil_div64(d->rows, strips), 64), reach);
   p.strips = (int)ceil_div64(d->rows, p.strip_rows);
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
   p.db_tiles = (int)ceil_div64(d->rows, q_side(p.gate_tile));
@@ -624,6 +629,7 @@ static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
   typedef GateSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
+  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d units are too many for one launch", (long long)a.rows, a.f);
   hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
@@ -640,6 +646,7 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
+  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
   hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
@@ -649,6 +656,7 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   typedef DwSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
+  SSMI_REQUIRE((int64_t)a.np * a.nq * strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
   hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;

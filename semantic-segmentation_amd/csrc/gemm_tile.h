@@ -25,6 +25,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char* lds_bytes;
 
+static constexpr int64_t kMostBlocks = 1 << 24;      // of 256 threads: a launch has fewer than 2^32 of them
+
 __device__ __forceinline__ unsigned spread_blocks(unsigned b, unsigned n) {      // workgroups of one XCD take consecutive tiles (a bijection of [0, n))
   const unsigned q = n >> 3, r = n & 7u, x = b & 7u;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel_cols(const uint8_t*
   if (col >= n || b >= nb) return;
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const unsigned e = scales[(int64_t)col * nb + b];
-  const float s = __builtin_bit_cast(float, e == 255u ? 0x7FC00000u : e << 23);
+  const float s = __builtin_bit_cast(float, e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);      // 0: 2^-127
   for (int q = 0; q < 4; ++q) {
     unsigned c = *reinterpret_cast<const unsigned*>(codes + ((int64_t)col * nb + b) * 16 + q * 4);
 #pragma unroll
@@ -440,6 +440,7 @@ static ssmi_status launch_tiles(Mx4Args a, hipStream_t st) {
   typedef Mx4Shape<SP, SQ, GATE> S;
   a.np = (unsigned)ceil_div64(a.n, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, S::kQ);
+  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "mx4: %lld rows of %d columns are too many for one launch", (long long)a.rows, a.n);
   hipLaunchKernelGGL((mx4_kernel<T, SP, SQ, GATE>), dim3(a.np * a.nq), dim3(256), S::kLds, st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;

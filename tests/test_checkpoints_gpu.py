@@ -140,3 +140,21 @@ def test_another_stream_and_captured_replays():
             torch.cuda.synchronize()
             assert torch.equal(out, y)
             assert torch.equal(cp.store_8bit(x).restore(), y)
+
+
+def test_offsets_past_32_bits():
+    """2.2e9 values: the last pixels keep what a call on them alone keeps."""
+    x = torch.zeros(70000000, 32, dtype=torch.bfloat16, device=DEV)
+    tail = _data(300, 32, torch.bfloat16, 4).to(DEV)
+    x[-300:] = tail
+    kept, small = cp.store_8bit(x), cp.store_8bit(tail)
+    assert torch.equal(kept.codes[-300:], small.codes) and torch.equal(kept.scales[-300:], small.scales)
+    y = kept.restore()
+    assert torch.equal(y[-300:], small.restore()) and not bool(y[:1000].any())
+
+
+@pytest.mark.parametrize("c", [1100, 2100, 4133])
+def test_more_groups_than_a_block_holds(c):
+    x = _data(37, c, torch.float32, c).to(DEV)
+    _check(x, cp.store_8bit(x))
+    _check(x.bfloat16(), cp.store_8bit(x.bfloat16()))

@@ -334,3 +334,48 @@ def test_layer():
     again = ff.GatedFeedForward2D(24, activation="gelu")
     again.set_weights(layer.get_weights())
     assert torch.equal(again(x.detach()), y.detach())
+
+
+def test_second_derivative_is_refused():
+    x = torch.randn(8, 16, device=DEV, requires_grad=True)
+    w = [torch.randn(16, 8, device=DEV, requires_grad=True) for _ in range(2)]
+    y = ff.gated_feed_forward(x, *w)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_relu_keeps_a_nan():
+    x = torch.randn(70, 16, device=DEV)
+    x[3, 2] = float("nan")
+    w = [torch.randn(16, 8, device=DEV) for _ in range(2)]
+    for rows in (70, 5):      # tiles, the kernel of few rows
+        y = ff.gated_feed_forward(x[:rows], *w, activation="relu")
+        assert bool(torch.isnan(y[3]).all()) and int(torch.isnan(y).sum()) == 8
+
+
+def test_weight_gradient_strips_past_two_gib():
+    """70000 x (2 * 16384) bfloat16 gradients of the projections: a strip of half the rows would pass 32-bit offsets.  The gradients of a
+    few units equal those of a call on these units alone up to the order of float32 sums (and one bfloat16 rounding of the results)."""
+    rows, c, f = 70000, 32, 16384
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(rows, c, generator=g, device=DEV).bfloat16()
+    w = [(torch.randn(c, f, generator=g, device=DEV) / c ** 0.5).bfloat16().requires_grad_() for _ in range(2)]
+    dy = torch.randn(rows, f, generator=g, device=DEV).bfloat16()
+    got = torch.autograd.grad(ff.gated_feed_forward(x, *w), w, dy)
+    for at in (0, 8192, 16384 - 64):
+        part = [t[:, at:at + 64].detach().clone().requires_grad_() for t in w]
+        want = torch.autograd.grad(ff.gated_feed_forward(x, *part), part, dy[:, at:at + 64])
+        for a, b in zip(got, want):
+            d = (a[:, at:at + 64].float() - b.float()).norm() / b.float().norm()
+            assert float(d) <= 2.0 ** -8
+
+
+def test_rows_past_two_gib():
+    rows, c, f = 2300000, 512, 16      # 2.36e9 bytes of input
+    x = torch.zeros(rows, c, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    tail = torch.randn(1000, c, generator=g, device=DEV).bfloat16()
+    x[-1000:] = tail
+    w = [(torch.randn(c, f, generator=g, device=DEV) / c ** 0.5).bfloat16() for _ in range(2)]
+    y = ff.gated_feed_forward(x, *w)
+    assert torch.equal(y[-1000:], ff.gated_feed_forward(tail, *w)) and not bool(y[:-1000].any())

@@ -95,7 +95,7 @@ def act64(name, g):
     return torch.relu(g) if name == "relu" else torch.sigmoid(g)
 
 
-SHAPES = [(1, 1, 1), (1, 32, 32), (1, 1000, 96), (2, 33, 31), (5, 300, 65), (16, 64, 33), (31, 1024, 40), (32, 96, 64), (33, 32, 1), (64, 64, 64), (100, 257, 130), (129, 1000, 67), (300, 288, 129),
+SHAPES = [(1, 1, 1), (1, 32, 32), (1, 1000, 96), (2, 33, 31), (5, 300, 65), (16, 64, 33), (31, 1024, 40), (32, 96, 64), (32, 2752, 33), (20, 5000, 40), (33, 32, 1), (64, 64, 64), (100, 257, 130), (129, 1000, 67), (300, 288, 129),
           (513, 40, 260)]
 
 
@@ -231,3 +231,25 @@ def test_train_in_8_bits_answer_in_4():
     assert float((got - want).norm() / want.norm()) <= 2e-6
     # and the quantisation itself: two operands off by at most half a step (1/8 of a value, less on average) each
     assert float((got - layer(x).detach().double().cpu().reshape(-1, 48)).norm() / want.norm()) <= 0.5
+
+
+def test_rows_past_two_gib():
+    rows, k = 1200000, 1024      # 2.46e9 bytes of bfloat16 input
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV)
+    tail = data(500, k, torch.bfloat16, 3).to(DEV)
+    x[-500:] = tail
+    q = ms.quantize_mx4_weights((data(k, 16, torch.float32, 4) / 32).to(DEV))
+    y = ms.mx4_dense(x, q)
+    assert torch.equal(y[-500:], ms.mx4_dense(tail, q)) and not bool(y[:-500].any())
+
+
+def test_exponents_of_other_programs():
+    """Codes made elsewhere may use every exponent that the format has: the values are those of the format."""
+    codes = torch.randint(0, 256, (5, 32), generator=torch.Generator().manual_seed(1), dtype=torch.uint8)
+    scales = torch.tensor([[0, 1], [15, 16], [127, 254], [200, 100], [120, 130]], dtype=torch.uint8)
+    w = ms.MX4Weights(codes.to(DEV), scales.to(DEV), 64).dequantize().double().cpu()
+    nib = torch.stack([codes & 15, codes >> 4], -1).reshape(5, 64)
+    v = torch.from_numpy(O.GRID4)[(nib & 7).long()] * torch.where(nib >= 8, -1.0, 1.0)
+    want = (v.reshape(5, 2, 32) * torch.ldexp(torch.ones(5, 2, dtype=torch.float64), scales.int() - 127)[..., None]).reshape(5, 64).t()
+    over = want.abs() > torch.finfo(torch.float32).max
+    assert torch.equal(w[~over], want[~over]) and bool(torch.isinf(w[over]).all())
