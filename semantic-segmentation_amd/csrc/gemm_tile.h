@@ -46,9 +46,11 @@ __device__ __forceinline__ TileAt tile_at(unsigned v, unsigned np, unsigned nq) 
 
 // 64 lanes x 16 bytes from buffer offsets to LDS bytes [at, at + 1024), `at` uniform.  In assembly because the compiler, which cannot
 // tell the two stages apart, would wait for every such load in front of the next LDS read; nothing is returned in registers, and the
-// tile loop waits for them itself (stage_wait, in order) in front of the barrier that publishes a stage.
+// tile loop waits for them itself (stage_wait, in order) in front of the barrier that publishes a stage.  The pause covers what M0 needs and
+// the five wait states of a scalar operand that a vector instruction wrote (a spilled one, read back): the compiler does not look into
+// assembly for them.
 __device__ __forceinline__ void stage16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, unsigned at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
 template <int LEFT>
 __device__ __forceinline__ void stage_wait() {      // until at most LEFT loads are on their way
