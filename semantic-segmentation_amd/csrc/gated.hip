@@ -502,21 +502,22 @@ static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 //   gate, dW: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
 //   dx:       256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192, else as above
 // float32 stays with the last two: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
-enum Tile { kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
+enum Tile { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 static Tile tile_for(int64_t q, int64_t p, bool wide, int64_t times = 1) {
   if (wide && ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
   return ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
 }
 static Tile tile_for_dx(int64_t rows, int64_t c, bool wide) {
   if (wide && c > 128 && ceil_div64(rows, 256) * ceil_div64(c, 256) >= 192) return kTile256x256;
-  return tile_for(rows, c, false);
+  const Tile t = tile_for(rows, c, false);
+  return t == kTile128x64 && ceil_div64(rows, 64) * ceil_div64(c, 128) < 384 ? kTile64x64 : t;
 }
 static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t most_strips) {
   // the larger tile only under strips of 4096 rows, where its own speed outweighs the partial sums of twice the strips
   if (wide && c > 128 && rows / ceil_div64(512, ceil_div64(p, 128) * ceil_div64(c, 256)) >= 4096) return kTile128x256;
   return tile_for(c, p, false, most_strips);
 }
-static inline int64_t q_side(Tile t) { return t == kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
+static inline int64_t q_side(Tile t) { return t <= kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
 
 struct GatePlan {
   int es, ce;                       // bytes of an activation, activations in 16 bytes
@@ -667,7 +668,8 @@ static ssmi_status launch_dx(Tile t, const GateDxArgs& a, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (t == kTile256x256) return launch_dx_as<T, 4, 4>(a, st);
   }
-  return t == kTile128x128 ? launch_dx_as<T, 2, 2>(a, st) : launch_dx_as<T, 2, 1>(a, st);
+  if (t == kTile128x128) return launch_dx_as<T, 2, 2>(a, st);
+  return t == kTile128x64 ? launch_dx_as<T, 2, 1>(a, st) : launch_dx_as<T, 1, 1>(a, st);
 }
 template <typename T>
 static ssmi_status launch_dw(Tile t, const GateDwArgs& a, int strips, hipStream_t st) {
