@@ -11,7 +11,7 @@
 // The passes move bytes and nothing else binds them: a lane owns 16 bytes of a pixel (eight bfloat16 or four float32 channels, so that a
 // wave's accesses are whole lines), four or eight lanes share a group, and the group's maximum is two or three cross-lane steps on the
 // integer patterns of |x| (which order as the values do and put infinities and NaN on top).
-// Measured: store + restore of 1M x 64 bfloat16 pixels 40 us, 5.2 TB/s of the 407 MB that they move (a large copy: 5.2 TB/s).
+// Measured: store + restore of 1M x 64 bfloat16 pixels 77 us, 5.3 TB/s of the 407 MB that they move (a large copy: 5.2 TB/s).
 #include "common.h"
 
 namespace ssmi {

@@ -5,6 +5,8 @@
 // byte each, a quarter of bfloat16's) for few.
 // Quantisation: s = the smallest power of two >= 2^-111 with max |x| < 7 s, values rounded to nearest even (v_cvt_scalef32_pk_fp4).
 #include "gemm_tile.h"
+#include <algorithm>
+
 #include "gate_act.h"
 
 namespace ssmi {
@@ -403,10 +405,12 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(const T* __restrict__ x, 
 
 static inline bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline int blocks_of(int k) { return (k + kBlock - 1) / kBlock; }
-static constexpr int kFewRows = 32;                        // one matrix instruction's rows
 static constexpr size_t kFewBytes = 48 * 1024;             // of quantised x in LDS
 static inline size_t few_bytes(int64_t rows, int nb) { return (size_t)rows * (17 * (size_t)nb + 16); }
-static inline bool takes_few(int64_t rows, int k) { return rows <= kFewRows && few_bytes(rows, blocks_of(k)) <= kFewBytes; }
+// mx4_rows_kernel saves the launch that quantises x, but each of its workgroups quantises all of it: it pays up to 8 rows, and 6144 values more,
+// of at most the 32 that a matrix instruction takes.  Its and the tiles' times in us, quantisation included: 1 x 512 -> 512 5.2 and 7.2,
+// 16 x 512 7.1 and 7.6, 32 x 512 9.1 and 7.8; 8 x 2048 -> 2048 10.2 and 11.9, 16 x 2048 13.8 and 12.1; 32 x 96 -> 301 6.1 and 8.4.
+static inline bool takes_few(int64_t rows, int k) { return rows <= std::min(32, 8 + 6144 / k) && few_bytes(rows, blocks_of(k)) <= kFewBytes; }
 static inline size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 static ssmi_status check_mx4(const char* who, int64_t rows, int32_t k, int32_t n, int64_t ld, int32_t dtype) {

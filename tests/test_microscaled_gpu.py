@@ -99,8 +99,12 @@ SHAPES = [(1, 1, 1), (1, 32, 32), (1, 1000, 96), (2, 33, 31), (5, 300, 65), (16,
           (513, 40, 260)]
 
 
+# the borders between the kernel of few rows and the tiles: 32 rows, fewer for a long reduction
+BORDERS = [(9, 6144, 33), (10, 6144, 33), (14, 1000, 40), (15, 1000, 40), (20, 512, 64), (21, 512, 64), (8, 16384, 5), (1, 65536, 3)]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,k,n", SHAPES)
+@pytest.mark.parametrize("rows,k,n", SHAPES + BORDERS)
 def test_dense_and_gated(rows, k, n, dtype):
     x = data(rows, k, dtype, rows + k + n, spread=0.5)
     w = [data(k, n, torch.float32, 5 + i + k, spread=0.3) / math.sqrt(k) for i in range(2)]
