@@ -18,7 +18,7 @@ __device__ __forceinline__ float gate_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-v));      // exp = inf gives 0
 }
 // Phi(g) = (1 + erf(g / sqrt 2)) / 2, and exp(-g^2 / 2) beside it.  bfloat16: Abramowitz and Stegun 7.1.26, whose own exponential is the
-// density's - erf off by at most 1.5e-7, one reciprocal, one exponential, seven multiply-adds (the library's erff costs four times that
+// density's - erf off by at most 1.5e-7, one reciprocal, one exponential, seven multiply-adds (the library's erff costs far more instructions
 // and the registers of both its branches); float32: the library's.
 template <typename T>
 __device__ __forceinline__ float gate_phi(float g, float& density) {

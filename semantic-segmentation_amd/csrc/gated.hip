@@ -22,7 +22,7 @@ __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
 // Stages, K step, q rows that the epilogue takes at once and workgroups to a CU (registers and LDS) of a tile shape.  The products of dx
 // and dW run long K loops: 128-byte steps, fewer barriers (16k x 512 -> 2048: dx 65 us, with 64-byte steps 92).  The gate kernels run
 // short ones with an epilogue as long: the 128 x 128 tile takes 64-byte steps and a quarter of the tile through LDS at a time, so three
-// workgroups share a CU and one's epilogue runs under the others' products (10k x 256 -> 688 with dg, du: 24.4 -> 20.5 us).
+// workgroups share a CU and one's epilogue runs under the others' products.
 template <int SP, int SQ>
 struct ProductShape {
   static constexpr int kStep = SP * SQ == 8 ? 64 : 128, kStages = SP * SQ == 8 ? 3 : 2, kAtOnce = SQ > 2 ? 2 : SQ;
@@ -42,7 +42,7 @@ struct GateArgs {
   void* out;                    // y, or [dg | du]
   int64_t rows, x_ld, w_ld, out_ld, dy_ld;
   int c, f, fp;                 // fp: units with the padding that [dg | du] rows have
-  int act, bf_params, vec_out, vec_dy;
+  int act, bf_params, vec_out, vec_dy;      // see vec_of
   int split;                    // backward: [dg | du] as two bfloat16 terms each, [dg | du | rest of dg | rest of du]
   float* db;                    // backward: column sums of [dg | du] per row tile, or nullptr
   unsigned np, nq;
@@ -144,6 +144,38 @@ __global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(
         v[e] = dy[e] * h;
       }
     };
+    if constexpr (sizeof(T) == 2 && !BWD) {
+      // The forward pass stores straight from the accumulators: no LDS, no barrier, 32 bytes of a row at a time (64k x 512 -> 2048: 385 ->
+      // 371 us, 16k rows 83 -> 74).  Where dy has to come the same way, or nothing but the store is to do (dx), whole rows through LDS
+      // are faster (64k x 512 -> 2048 with dg, du: 421 against 476 us; 16k rows, dx: 66 against 72).
+      if (whole && a.vec_out == 2) {
+        const int hh = lane >> 5, u0 = wp * (SP / 2) * 32;
+        T* const y = out + (int64_t)(s.wq * SQ * 32) * a.out_ld + u0;
+        const unsigned y_lane = (unsigned)(lane & 31) * (unsigned)a.out_ld;
+#pragma unroll
+        for (int i = 0; i < SP / 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            float bg8[8] = {}, bu8[8] = {};
+            if (a.bg) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int unit = f0 + u0 + i * 32 + 8 * (k + e / 4) + 4 * hh + e % 4;
+                bg8[e] = param_at(a.bg, a.bf_params, unit);
+                bu8[e] = param_at(a.bu, a.bf_params, unit);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) {
+              f32x4 o[2];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = gate_act<T, kAct>(acc[i][j][4 * k + e] + bg8[e]) * (acc[i + SP / 2][j][4 * k + e] + bu8[e]);
+              put8(y + j * 32 * a.out_ld + i * 32 + 8 * k + y_lane, hh, o[0], o[1]);
+            }
+          }
+        return;
+      }
+    }
     if (whole) {
       typename Act<T>::raw4 dy[BWD ? R::kRounds : 1];
       R::template run<R::kRounds>(
@@ -409,77 +441,87 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadJobs jobs) {
 }
 
 // A few rows: bound by reading the weights (or by latency), so no tiles and no staging of W.  A workgroup owns 32 units of both
-// projections; 32 threads stand side by side in k for each four units and add their sums at the end.
-template <typename T, typename P, int MB, bool VEC>
-__global__ __launch_bounds__(256) void gate_rows_kernel(GateArgs a) {
-  extern __shared__ float xs[];                     // [MB][c]
-  __shared__ float red[4][8][MB][8];
+// projections.  Four lanes side by side hold eight units each, 16 bytes of bfloat16 or twice 16 of float32; the other 16 WAVES of them share
+// the channels, so that all loads of a short reduction are on their way at once.
+template <typename P, bool VEC>
+__device__ __forceinline__ void fetch8(const P* p, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(P) == 2) {
+      const u32x4 r = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = __uint_as_float(r[e] << 16);
+        v[2 * e + 1] = __uint_as_float(r[e] & 0xFFFF0000u);
+      }
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+// sums over the lanes that differ in bit 5, then 4, 3 and 2; each step sends half of the values and keeps the other, so lane 4 s + oct ends
+// with the N / 16 values from s N / 16 on
+template <int N, int BIT>
+__device__ __forceinline__ void fold(float* v, int lane) {
+  const bool up = lane & BIT;
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float keep = up ? v[N / 2 + i] : v[i], send = up ? v[i] : v[N / 2 + i];
+    v[i] = keep + __shfl_xor(send, BIT, 64);
+  }
+  if constexpr (BIT > 4) fold<N / 2, BIT / 2>(v, lane);
+}
+template <typename T, typename P, int MB, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES) void gate_rows_kernel(GateArgs a) {
+  extern __shared__ float xs[];                     // [c][MB]
+  __shared__ float red[WAVES][MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m0 = (int64_t)blockIdx.y * MB;
   const int nm = (int)min((int64_t)MB, a.rows - m0);
-  for (int i = threadIdx.x; i < MB * a.c; i += 256) {
-    const int m = i / a.c, k = i - m * a.c;
-    xs[i] = m < nm ? Act<T>::gld(static_cast<const T*>(a.x) + (m0 + m) * a.x_ld + k) : 0.f;
+  for (int k = threadIdx.x; k < a.c; k += 64 * WAVES) {
+    float x[MB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) x[m] = Act<T>::gld(static_cast<const T*>(a.x) + (m0 + min(m, nm - 1)) * a.x_ld + k);      // all on their way at once
+#pragma unroll
+    for (int m = 0; m < MB; ++m) xs[k * MB + m] = x[m];      // rows behind the last repeat it and are not written
   }
   __syncthreads();
-  const int quad = lane & 7, slice = wave * 8 + (lane >> 3);
-  const int f = blockIdx.x * 32 + quad * 4;
+  const int oct = lane & 3, f = blockIdx.x * 32 + oct * 8, n = a.f - f;
   const P *wg = static_cast<const P*>(a.wg) + f, *wu = static_cast<const P*>(a.wu) + f;
-  float sg[MB][4], su[MB][4];
+  float sum[16 * MB];      // [side][unit][row]
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sg[m][e] = su[m][e] = 0.f;
-  const int n = a.f - f;
+  for (int i = 0; i < 16 * MB; ++i) sum[i] = 0.f;
   if (n > 0) {
-#pragma unroll 4
-    for (int k = slice; k < a.c; k += 32) {
-      float g[4], u[4];
-      fetch4<P>(wg + (int64_t)k * a.f, g, n, VEC);
-      fetch4<P>(wu + (int64_t)k * a.f, u, n, VEC);
-      if constexpr (sizeof(P) != sizeof(T)) {      // float32 parameters under bfloat16 activations are multiplied as bfloat16
+#pragma unroll(sizeof(P) == 2 ? 4 : 2)      // 32 registers of loads
+    for (int k = wave * 16 + (lane >> 2); k < a.c; k += 16 * WAVES) {
+      float w[2][8];
+      fetch8<P, VEC>(wg + (int64_t)k * a.f, n, w[0]);
+      fetch8<P, VEC>(wu + (int64_t)k * a.f, n, w[1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { g[e] = (float)(T)g[e]; u[e] = (float)(T)u[e]; }
-      }
+      for (int i = 0; i < 16; ++i) {
+        // float32 parameters under bfloat16 activations are multiplied as bfloat16
+        const float wv = sizeof(P) != sizeof(T) ? (float)(T)w[i / 8][i % 8] : w[i / 8][i % 8];
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const float xv = xs[m * a.c + k];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sg[m][e] = fmaf(xv, g[e], sg[m][e]);
-          su[m][e] = fmaf(xv, u[e], su[m][e]);
-        }
+        for (int m = 0; m < MB; ++m) sum[i * MB + m] = fmaf(xs[k * MB + m], wv, sum[i * MB + m]);
       }
     }
   }
+  fold<16 * MB, 32>(sum, lane);
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-      for (int o = 8; o < 64; o <<= 1) {
-        sg[m][e] += __shfl_xor(sg[m][e], o, 64);
-        su[m][e] += __shfl_xor(su[m][e], o, 64);
-      }
-    }
-  if (lane < 8) {
-#pragma unroll
-    for (int m = 0; m < MB; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        red[wave][lane][m][e] = sg[m][e];
-        red[wave][lane][m][4 + e] = su[m][e];
-      }
-  }
+  for (int m = 0; m < MB; ++m) red[wave][m][(lane >> 5) * 32 + oct * 8 + ((lane >> 2) & 7)] = sum[m];
   __syncthreads();
-  for (int i = threadIdx.x; i < nm * 32; i += 256) {
+  for (int i = threadIdx.x; i < nm * 32; i += 64 * WAVES) {
     const int m = i >> 5, col = i & 31, ff = blockIdx.x * 32 + col;
     if (ff >= a.f) continue;
     float g = 0.f, u = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      g += red[w][col >> 2][m][col & 3];
-      u += red[w][col >> 2][m][4 + (col & 3)];
+    for (int w = 0; w < WAVES; ++w) {
+      g += red[w][m][col];
+      u += red[w][m][32 + col];
     }
     if (a.bg) {
       g += param_at(a.bg, a.bf_params, ff);
@@ -492,16 +534,15 @@ __global__ __launch_bounds__(256) void gate_rows_kernel(GateArgs a) {
 
 // --------------------------------------------------------------------------------------------------------------- host side
 
-static constexpr int kRowsKernelMost = 16;              // rows that gate_rows_kernel takes (see ssmi_gated_ff_fwd)
-static constexpr int kRowsKernelChannels = 2048;        // its x rows have to fit LDS: 4 x 2048 floats
-
 static inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
-//   gate, dW: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
-//   dx:       256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192, else as above
-// float32 stays with the last two: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
+//   gate: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
+//   dx:   256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192; 64 x 64 where 128 x 64
+//         makes under 384 (4096 x 512 -> 2048 bfloat16 41 -> 36 us, 16k x 128 -> 512 float32 49 -> 47); else as above
+//   dW:   128 x 256 under strips of 4096 rows; else as above, counting the strips
+// float32 takes no wide tiles: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
 enum Tile { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 static Tile tile_for(int64_t q, int64_t p, bool wide, int64_t times = 1) {
   if (wide && ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
@@ -544,9 +585,9 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
   p.w_bytes = p.pad_w ? 2 * up256((size_t)d->c * p.fp * p.es) : 0;
   p.x_bytes = p.pad_x ? up256((size_t)d->rows * p.cp * p.es) : 0;
-  // One bfloat16 of dg and du is off by 2^-9 on average and shows beside the output's own rounding; two are exact to 2^-17 and cost the two
-  // products that read them twice the arithmetic: nothing below 2^27 multiplications, where launches and latency decide (the backward
-  // pass of 102 x 893 -> 391: 45 us either way), half as much time again above (16k x 512 -> 2048: 260 against 430 us).
+  // One bfloat16 of dg and du is off by up to 2^-9 and shows beside the output's own rounding; two are exact to 2^-17 and cost the two
+  // products that read them twice the arithmetic: some ten us up to 2^27 multiplications (the backward pass of 102 x 893 -> 391: 35 us with
+  // one term, 43 with two; 512 x 512 -> 512: 26 and 38), too much above (4096 x 256 -> 1024: 48 and 72; 16k x 512 -> 2048: 247 and 440).
   p.split = bf && (double)d->rows * d->c * d->f <= (double)(1 << 27);
   p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, bf && !p.split);      // the wide tile's epilogue has no registers for the second terms
   p.dgu_bytes = up256((size_t)d->rows * (p.split ? 4 : 2) * p.fp * p.es);
@@ -583,6 +624,9 @@ static ssmi_status check_desc(const char* who, const ssmi_gated_desc* d) {
 }
 
 static inline bool aligned(const void* p, int b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
+
+// how rows may be stored: 0 value by value, 1 four values at a time, 2 eight
+static inline int vec_of(int64_t ld, const void* p, int es) { return ld % 4 || !aligned(p, 4 * es) ? 0 : ld % 8 || !aligned(p, 16) ? 1 : 2; }
 
 // operands in the tile engine's form, padded copies in ws where they are not in it already
 struct Staged {
@@ -681,23 +725,30 @@ static ssmi_status launch_dw(Tile t, const GateDwArgs& a, int strips, hipStream_
 
 template <typename T, typename P, int MB>
 static void launch_rows_mb(const GateArgs& a, bool vec, hipStream_t st) {
-  const dim3 grid((unsigned)ceil_div64(a.f, 32), (unsigned)ceil_div64(a.rows, MB));
+  constexpr int kWaves = MB <= 2 ? 16 : 8;
+  const dim3 grid((unsigned)ceil_div64(a.f, 32), (unsigned)ceil_div64(a.rows, MB)), block(64 * kWaves);
   const size_t lds = (size_t)MB * a.c * 4;
-  if (vec) hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, true>), grid, dim3(256), lds, st, a);
-  else hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, false>), grid, dim3(256), lds, st, a);
+  if (vec) hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, kWaves, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((gate_rows_kernel<T, P, MB, kWaves, false>), grid, block, lds, st, a);
 }
 template <typename T, typename P>
 static ssmi_status launch_rows(const GateArgs& a, hipStream_t st) {
-  const bool vec = a.f % 4 == 0 && aligned(a.wg, 4 * sizeof(P)) && aligned(a.wu, 4 * sizeof(P));
+  const bool vec = a.f % 8 == 0 && aligned(a.wg, 16) && aligned(a.wu, 16);
   if (a.rows == 1) launch_rows_mb<T, P, 1>(a, vec, st);
-  else if (a.rows == 2) launch_rows_mb<T, P, 2>(a, vec, st);
+  else if (a.rows == 2 || sizeof(P) == 2) launch_rows_mb<T, P, 2>(a, vec, st);      // bfloat16 parameters: see takes_rows_kernel
   else if (a.rows <= 4) launch_rows_mb<T, P, 4>(a, vec, st);
-  else launch_rows_mb<T, P, 4>(a, vec, st);
+  else launch_rows_mb<T, P, 8>(a, vec, st);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
 
-static bool takes_rows_kernel(const ssmi_gated_desc* d) { return d->rows <= kRowsKernelMost && d->c <= kRowsKernelChannels; }
+// Rows that gate_rows_kernel takes: as many as it beats the tiles at.  Its and their times in us, bfloat16: 1 x 512 -> 2048 3.9 and 5.9, 2 rows
+// 4.7 and 5.9, 4 rows 6.1 and 5.9, 1 x 2048 -> 4096 14 and 19.  Under float32 parameters the tiles need a bfloat16 copy of them first (1 x 512
+// -> 2048 4.2 and 12.5, 16 rows 8.7 and 12.5), and in float32 they cannot hide a long reduction (1 row 4.0 and 20, 24 rows 9.8 and 20.6,
+// 48 rows 17 and 21).  Its rows of x have to fit LDS: eight of 2048 float32.
+static bool takes_rows_kernel(const ssmi_gated_desc* d) {
+  return d->rows <= (d->param_dtype == SSMI_BF16 ? 2 : d->dtype == SSMI_BF16 ? 16 : 32) && d->c <= 2048;
+}
 
 template <typename T>
 static ssmi_status gated_fwd(const ssmi_gated_desc* d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, void* y, void* ws,
@@ -707,14 +758,16 @@ static ssmi_status gated_fwd(const ssmi_gated_desc* d, const void* x, const void
   a.bf_params = d->param_dtype == SSMI_BF16;
   if (takes_rows_kernel(d)) {
     a.x = x; a.wg = wg; a.wu = wu; a.x_ld = d->x_ld;
-    if (a.bf_params) return launch_rows<T, bf16>(a, st);
+    if constexpr (sizeof(T) == 2) {
+      if (a.bf_params) return launch_rows<T, bf16>(a, st);
+    }
     return launch_rows<T, float>(a, st);
   }
   const GatePlan p = gate_plan(d);
   const Staged s = stage_operands<T>(d, p, x, wg, wu, ws, st);
   SSMI_LAUNCH_CHECK();
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.fp = p.fp;
-  a.vec_out = d->y_ld % 4 == 0 && aligned(y, 4 * p.es);
+  a.vec_out = vec_of(d->y_ld, y, p.es);
   return launch_gate<T, false>(p.gate_tile, a, st);
 }
 
@@ -734,14 +787,14 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = sides * (int64_t)p.fp; a.dy_ld = d->y_ld;
   a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf; a.split = p.split;
   a.db = dbg || dbu ? dbp : nullptr;
-  a.vec_out = 1;
-  a.vec_dy = d->y_ld % 4 == 0 && aligned(dy, 4 * p.es);
+  a.vec_out = 2;      // rows of whole 16 bytes
+  a.vec_dy = vec_of(d->y_ld, dy, p.es);
   ssmi_status r = launch_gate<T, true>(p.gate_tile, a, st);
   if (r != SSMI_OK) return r;
   if (dx) {
     GateDxArgs b = {};
     b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp; b.sides = sides;
-    b.vec_out = d->x_ld % 4 == 0 && aligned(dx, 4 * p.es);
+    b.vec_out = vec_of(d->x_ld, dx, p.es);
     r = launch_dx<T>(p.dx_tile, b, st);
     if (r != SSMI_OK) return r;
   }

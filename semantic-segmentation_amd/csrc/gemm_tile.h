@@ -330,4 +330,15 @@ __device__ __forceinline__ void fetch4(const T* p, float (&v)[4], int n, bool ve
   }
 }
 
+// Sixteen consecutive bfloat16 columns of a row straight from the accumulator layout: the row's lower lane (hh = 0) holds columns 0-3 (`a`)
+// and 8-11 (`b`), the upper one 4-7 and 12-15.  One swap of the wave's halves brings each lane eight of them: a 16-byte store, 32 bytes a
+// row.
+__device__ __forceinline__ void put8(bf16* row, int hh, f32x4 a, f32x4 b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  auto pair = [](float x, float y) __attribute__((always_inline)) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{x, y}), bf16x2)); };
+  const auto p = __builtin_amdgcn_permlane32_swap(pair(a[0], a[1]), pair(b[0], b[1]), false, false);
+  const auto q = __builtin_amdgcn_permlane32_swap(pair(a[2], a[3]), pair(b[2], b[3]), false, false);
+  *reinterpret_cast<u32x4*>(row + 8 * hh) = u32x4{p[0], q[0], p[1], q[1]};
+}
 }  // namespace ssmi

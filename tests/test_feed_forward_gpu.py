@@ -113,6 +113,28 @@ def test_forward(rows, c, f, dtype, pdtype):
         close(got, y, err, "{} {}".format("bf16" if dtype == torch.bfloat16 else "f32", act))
 
 
+@pytest.mark.parametrize("dtype,pdtype", TYPES)
+@pytest.mark.parametrize("c,f", [(48, 64), (20, 36), (7, 33), (2048, 40), (2049, 40)])
+def test_every_count_of_few_rows(c, f, dtype, pdtype):
+    """The borders between the kernel of few rows (1, 2, 4 or 8 at a time) and the tiles; more channels than it takes."""
+    for rows in (1, 2, 3, 4, 7, 8, 9, 15, 16, 17, 31, 32, 33):
+        x, ws, bs, _ = make(rows, c, f, dtype, pdtype, rows % 2 == 1, rows + c + f)
+        y, err, _, _ = reference(x, ws, bs, None, "swish", dtype)
+        got = ff.gated_feed_forward(x.to(DEV), *(w.to(DEV) for w in ws), *(None if b is None else b.to(DEV) for b in bs), activation="swish")
+        close(got, y, err, "{} {} rows".format("bf16" if dtype == torch.bfloat16 else "f32", rows))
+
+
+@pytest.mark.parametrize("dtype,pdtype", TYPES)
+@pytest.mark.parametrize("rows,f", [(256, 128), (200, 132), (256, 130), (193, 129), (20000, 264)])
+def test_whole_and_cut_tiles_with_rows_of_every_alignment(rows, f, dtype, pdtype):
+    """Rows of y at 16, 8, 4 and 2 (or 4) bytes, with biases and without."""
+    for bias, act in ((True, "gelu"), (False, "sigmoid")):
+        x, ws, bs, _ = make(rows, 40, f, dtype, pdtype, bias, rows + f)
+        y, err, _, _ = reference(x, ws, bs, None, act, dtype)
+        got = ff.gated_feed_forward(x.to(DEV), *(w.to(DEV) for w in ws), *(None if b is None else b.to(DEV) for b in bs), activation=act)
+        close(got, y, err, "{} {}".format("bf16" if dtype == torch.bfloat16 else "f32", act))
+
+
 def run_own(x, ws, bs, dy, act, checkpoint=None):
     leaves = [t.to(DEV).requires_grad_() for t in [x, *ws, *(b for b in bs if b is not None)]]
     pair = leaves[3:] if len(leaves) == 5 else [None, None]
