@@ -243,12 +243,15 @@ __global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(
 }
 
 // dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection (and again
-// over the second terms of a split [dg | du])
+// over the second terms of a split [dg | du]).  Few tiles under a long K share it in strips, whose float32 sums [strip][rows][c4] are added
+// in their order by the reduction behind dW.
 struct GateDxArgs {
   const void *dgu, *wg, *wu;
   void* dx;
+  float* part;      // more than one strip: instead of dx
   int64_t rows, w_ld, dx_ld;
   int c, fp, vec_out, sides;      // sides: 2, or 4 when split
+  int each, strips, c4;           // K steps of a strip
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
@@ -262,10 +265,10 @@ struct DxSides : ProductShape<SP, SQ> {
   __amdgpu_buffer_rsrc_t wu;
   typename W::Reader rw;
   typename D::Reader rd;
-  int fp, half, sides, wp, wq;
-  __device__ __forceinline__ void one(lds_bytes s, int t, int j) const {
-    const int side = t >= 2 * half ? (t >= 3 * half ? 3 : 2) : t >= half ? 1 : 0;
-    const int ts = t - side * half, left = t < sides * half ? fp - ts * W::kStepK : 0;
+  int fp, half, first, end, wp, wq;      // the strip's steps
+  __device__ __forceinline__ void one(lds_bytes s, int step, int j) const {
+    const int t = first + step, side = t >= 2 * half ? (t >= 3 * half ? 3 : 2) : t >= half ? 1 : 0;
+    const int ts = t - side * half, left = t < end ? fp - ts * W::kStepK : 0;
     if (j < W::kLoads) {
       W w = wg;
       if (side & 1) w.rsrc = wu;
@@ -282,13 +285,15 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_k
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   typedef DxSides<T, SP, SQ> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const TileAt at = tile_at(spread_blocks(blockIdx.x, gridDim.x), a.np, a.nq);
+  const unsigned v = spread_blocks(blockIdx.x, gridDim.x), tiles = a.np * a.nq, strip = __builtin_amdgcn_readfirstlane(v / tiles);
+  const TileAt at = tile_at(v - strip * tiles, a.np, a.nq);
   const int64_t m0 = (int64_t)at.q * (SQ * 64);
   const int c0 = at.p * (SP * 64);
   S s;
   s.fp = a.fp;
-  s.sides = a.sides;
   s.half = (a.fp + S::W::kStepK - 1) / S::W::kStepK;
+  s.first = (int)strip * a.each;
+  s.end = min(s.first + a.each, a.sides * s.half);
   s.wp = wave >> 1;
   s.wq = wave & 1;
   s.wg.init(static_cast<const T*>(a.wg) + c0 * a.w_ld, a.w_ld, a.c - c0);
@@ -297,11 +302,16 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_k
   s.rw.init(lane);
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
-  tile_product<T, SP, SQ>(s, (lds_bytes)smem, a.sides * s.half, acc);
+  tile_product<T, SP, SQ>(s, (lds_bytes)smem, s.end - s.first, acc);
   typedef TileRows<SP, SQ, SP * 64, S::kAtOnce> R;
   const int wp = s.wp, c = c0 + R::col();
   auto pos = [&](int i) __attribute__((always_inline)) { return (wp * SP + i) * 32; };
-  if (m0 + SQ * 64 <= a.rows && c0 + SP * 64 <= a.c && a.vec_out) {
+  if (a.part) {
+    float* const part = a.part + (strip * a.rows + m0 + R::first()) * a.c4 + c;
+    R::template run<1>(acc, reinterpret_cast<float*>(smem), s.wq, pos, [](int) {}, [&](const float* row, int qc, int) __attribute__((always_inline)) {
+      if (m0 + R::first() + qc < a.rows && c < a.c) *reinterpret_cast<f32x4*>(part + (int64_t)qc * a.c4) = *reinterpret_cast<const f32x4*>(row);
+    });
+  } else if (m0 + SQ * 64 <= a.rows && c0 + SP * 64 <= a.c && a.vec_out) {
     T* const dx = static_cast<T*>(a.dx) + m0 * a.dx_ld + c0;
     const unsigned lane_at = (unsigned)R::first() * (unsigned)a.dx_ld + (unsigned)R::col();
     R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), s.wq, pos, [](int) {}, [&](const float* row, int qc, int) __attribute__((always_inline)) {
@@ -378,14 +388,41 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dw_k
                               });
 }
 
-// dW = sum of the strips' partial sums in their order, db = that of the row tiles' column sums; four units a thread, the bias row last
+// sum of n partial sums of four values in their order, eight on their way at a time
+__device__ __forceinline__ f32x4 ordered_sum(const float* s, int n, int64_t step) {
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  int k = 0;
+  for (; k + 8 <= n; k += 8) {
+    f32x4 v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[e];
+  }
+  for (; k < n; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
+  return sum;
+}
+// dW = sum of the strips' partial sums in their order, db = that of the row tiles' column sums; four units a thread, the bias row last;
+// behind them dx, where its sums lie in strips
 struct ReduceArgs {
-  const float *part, *db;
-  void *dwg, *dwu, *dbg, *dbu;
-  int64_t c;
+  const float *part, *db, *dx_part;
+  void *dwg, *dwu, *dbg, *dbu, *dx;
+  int64_t c, rows, dx_ld;
   int strips, db_tiles, f, fp, bf;
+  int dx_strips, dx_c, c4, dx_vec;
+  unsigned dw_blocks;
 };
+template <typename T>
 __global__ __launch_bounds__(256) void gate_reduce_kernel(ReduceArgs a) {
+  if (blockIdx.x >= a.dw_blocks) {
+    const int64_t i = (int64_t)(blockIdx.x - a.dw_blocks) * 256 + threadIdx.x, m = i / (a.c4 / 4);
+    const int c = (int)(i - m * (a.c4 / 4)) * 4;
+    if (m >= a.rows) return;
+    const f32x4 v = ordered_sum(a.dx_part + m * a.c4 + c, a.dx_strips, a.rows * a.c4);
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    store4<T>(static_cast<T*>(a.dx) + m * a.dx_ld + c, o, a.dx_c - c, a.dx_vec);
+    return;
+  }
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int quads = a.fp / 2;
   const int64_t ci = i / quads;
@@ -398,16 +435,7 @@ __global__ __launch_bounds__(256) void gate_reduce_kernel(ReduceArgs a) {
   const int n = bias ? a.db_tiles : a.strips;
   const int64_t step = (bias ? 1 : a.c) * 2 * a.fp;
   const float* s = bias ? a.db + p : a.part + ci * (2 * (int64_t)a.fp) + p;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  int k = 0;
-  for (; k + 8 <= n; k += 8) {      // eight on their way at a time
-    f32x4 v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[e];
-  }
-  for (; k < n; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
+  const f32x4 sum = ordered_sum(s, n, step);
   const int64_t at = (bias ? 0 : ci * a.f) + fu;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -496,7 +524,8 @@ __global__ __launch_bounds__(64 * WAVES) void gate_rows_kernel(GateArgs a) {
 #pragma unroll
   for (int i = 0; i < 16 * MB; ++i) sum[i] = 0.f;
   if (n > 0) {
-#pragma unroll(sizeof(P) == 2 ? 4 : 2)      // 32 registers of loads
+    constexpr int kAhead = sizeof(P) == 2 ? 4 : 2;      // 32 registers of loads
+#pragma unroll kAhead
     for (int k = wave * 16 + (lane >> 2); k < a.c; k += 16 * WAVES) {
       float w[2][8];
       fetch8<P, VEC>(wg + (int64_t)k * a.f, n, w[0]);
@@ -558,6 +587,14 @@ static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t m
   if (wide && c > 128 && rows / ceil_div64(512, ceil_div64(p, 128) * ceil_div64(c, 256)) >= 4096) return kTile128x256;
   return tile_for(c, p, false, most_strips);
 }
+// K steps that a strip of dx takes: all of them, unless its smallest tiles leave half of the card idle; then two workgroups to a CU, each with
+// 256 bfloat16 or 128 float32 values at least.  Whole backward pass, one strip and so: 64 x 64 -> 4096 bfloat16 122 and 20 us, float32 205
+// and 25; 31 x 80 -> 944 42 and 17, 60 and 22; strips of four times as many values 23, 31, 23 and 31.
+static int dx_each(Tile t, int64_t rows, int64_t c, int steps) {
+  const int64_t tiles = ceil_div64(rows, 64) * ceil_div64(c, 64);
+  if (t != kTile64x64 || tiles > 256) return steps;
+  return (int)std::max<int64_t>(ceil_div64(steps, 512 / tiles), 512 / 128);      // steps of 128 bytes
+}
 static inline int64_t q_side(Tile t) { return t <= kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
 
 struct GatePlan {
@@ -569,7 +606,8 @@ struct GatePlan {
   int64_t strip_rows;
   bool split;                       // [dg | du] in two bfloat16 terms
   int db_tiles;
-  size_t w_bytes, x_bytes, dgu_bytes, part_bytes, db_bytes;
+  int dx_each, dx_strips, c4;
+  size_t w_bytes, x_bytes, dgu_bytes, part_bytes, db_bytes, dx_bytes;
 };
 
 static GatePlan gate_plan(const ssmi_gated_desc* d) {
@@ -604,6 +642,11 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.strip_rows = std::min(up_to(ceil_div64(d->rows, strips), 64), reach);
   p.strips = (int)ceil_div64(d->rows, p.strip_rows);
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
+  p.c4 = (int)up_to(d->c, 4);
+  const int steps = (p.split ? 4 : 2) * (int)ceil_div64(p.fp * p.es, ProductShape<1, 1>::kStep);
+  p.dx_each = dx_each(p.dx_tile, d->rows, d->c, steps);
+  p.dx_strips = (int)ceil_div64(steps, p.dx_each);
+  p.dx_bytes = p.dx_strips > 1 ? up256((size_t)p.dx_strips * d->rows * p.c4 * 4) : 0;
   p.db_tiles = (int)ceil_div64(d->rows, q_side(p.gate_tile));
   p.db_bytes = up256((size_t)p.db_tiles * 2 * p.fp * 4);
   return p;
@@ -691,8 +734,8 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
-  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
+  SSMI_REQUIRE((int64_t)a.np * a.nq * a.strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
+  hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)a.strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
 }
@@ -779,6 +822,7 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   void* const dgu = s.ws;
   float* const part = reinterpret_cast<float*>(s.ws + p.dgu_bytes);
   float* const dbp = reinterpret_cast<float*>(s.ws + p.dgu_bytes + p.part_bytes);
+  float* const dxp = dx && p.dx_strips > 1 ? reinterpret_cast<float*>(s.ws + p.dgu_bytes + p.part_bytes + p.db_bytes) : nullptr;
   const int bf = d->param_dtype == SSMI_BF16;
   GateArgs a = {};
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.bg = bg; a.bu = bu; a.dy = dy; a.out = dgu;
@@ -791,10 +835,12 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   a.vec_dy = vec_of(d->y_ld, dy, p.es);
   ssmi_status r = launch_gate<T, true>(p.gate_tile, a, st);
   if (r != SSMI_OK) return r;
+  const int dx_vec = vec_of(d->x_ld, dx, p.es);
   if (dx) {
     GateDxArgs b = {};
+    b.part = dxp; b.each = p.dx_each; b.strips = p.dx_strips; b.c4 = p.c4;
     b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp; b.sides = sides;
-    b.vec_out = vec_of(d->x_ld, dx, p.es);
+    b.vec_out = dx_vec;
     r = launch_dx<T>(p.dx_tile, b, st);
     if (r != SSMI_OK) return r;
   }
@@ -805,10 +851,14 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
     r = launch_dw<T>(p.dw_tile, b, p.strips, st);
     if (r != SSMI_OK) return r;
   }
-  if (dw || a.db) {
-    const ReduceArgs b = {part, a.db, dwg, dwu, dbg, dbu, dw ? d->c : 0, p.strips, p.db_tiles, d->f, p.fp, bf};
-    const int64_t threads = (b.c + (a.db ? 1 : 0)) * (p.fp / 2);
-    hipLaunchKernelGGL(gate_reduce_kernel, dim3((unsigned)ceil_div64(threads, 256)), dim3(256), 0, st, b);
+  if (dw || a.db || dxp) {
+    ReduceArgs b = {};
+    b.part = part; b.db = a.db; b.dwg = dwg; b.dwu = dwu; b.dbg = dbg; b.dbu = dbu; b.c = dw ? d->c : 0;
+    b.strips = p.strips; b.db_tiles = p.db_tiles; b.f = d->f; b.fp = p.fp; b.bf = bf;
+    b.dx_part = dxp; b.dx = dx; b.rows = d->rows; b.dx_ld = d->x_ld; b.dx_strips = p.dx_strips; b.dx_c = d->c; b.c4 = p.c4; b.dx_vec = dx_vec;
+    b.dw_blocks = (unsigned)ceil_div64((b.c + (a.db ? 1 : 0)) * (p.fp / 2), 256);
+    const unsigned dx_blocks = dxp ? (unsigned)ceil_div64(d->rows * (p.c4 / 4), 256) : 0;
+    hipLaunchKernelGGL((gate_reduce_kernel<T>), dim3(b.dw_blocks + dx_blocks), dim3(256), 0, st, b);
     SSMI_LAUNCH_CHECK();
   }
   return SSMI_OK;
@@ -824,7 +874,7 @@ size_t ssmi_gated_ff_workspace_bytes(const ssmi_gated_desc* d, int32_t backward)
   if (check_desc("gated_ff_workspace_bytes", d) != SSMI_OK) return 0;
   const GatePlan p = gate_plan(d);
   if (!backward) return takes_rows_kernel(d) ? 0 : p.w_bytes + p.x_bytes;
-  return p.w_bytes + p.x_bytes + p.dgu_bytes + p.part_bytes + p.db_bytes;
+  return p.w_bytes + p.x_bytes + p.dgu_bytes + p.part_bytes + p.db_bytes + p.dx_bytes;
 }
 
 ssmi_status ssmi_gated_ff_fwd(const ssmi_gated_desc* d, const void* x, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* y,

@@ -206,6 +206,20 @@ def test_8bit_checkpoint_gives_the_gradients_at_the_restored_input(dtype):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype,pdtype", TYPES)
+@pytest.mark.parametrize("rows,c,f", [(1, 3, 1500), (31, 80, 944), (64, 64, 4096), (130, 33, 1000), (1100, 72, 2056)])
+def test_input_gradient_over_many_units(rows, c, f, dtype, pdtype):
+    """Few tiles under a long sum: dx in strips, with the kernels' gradients and alone."""
+    x, ws, bs, dy = make(rows, c, f, dtype, pdtype, rows % 2 == 0, rows + c + f)
+    _, _, want, err = reference(x, ws, bs, dy, "swish", dtype)
+    _, got = run_own(x, ws, bs, dy, "swish")
+    for g, w, e, name in zip(got, want, err, ("dx", "dwg", "dwu", "dbg", "dbu")):
+        close(g, w, e, "{} {}".format("bf16" if dtype == torch.bfloat16 else "f32", name))
+    leaf = x.to(DEV).requires_grad_()
+    y = ff.gated_feed_forward(leaf, *(w.to(DEV) for w in ws), *(None if b is None else b.to(DEV) for b in bs), activation="swish")
+    assert torch.equal(torch.autograd.grad(y, leaf, dy.to(DEV))[0], got[0])
+
+
 @pytest.mark.parametrize("dtype,rows,c,f", [(torch.bfloat16, 33000, 64, 192), (torch.float32, 33000, 64, 192), (torch.bfloat16, 4099, 1000, 1500), (torch.float32, 8200, 264, 520)])
 def test_sizes_that_take_the_large_tiles(dtype, rows, c, f):
     x, ws, bs, dy = make(rows, c, f, dtype, dtype, True, 3)
