@@ -388,16 +388,23 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dw_k
                               });
 }
 
-// sum of n partial sums of four values in their order, eight on their way at a time
+// sum of n partial sums of four values in their order, sixteen on their way at a time
 __device__ __forceinline__ f32x4 ordered_sum(const float* s, int n, int64_t step) {
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   int k = 0;
-  for (; k + 8 <= n; k += 8) {
-    f32x4 v[8];
+  for (; k + 16 <= n; k += 16) {
+    f32x4 v[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
+    for (int e = 0; e < 16; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[e];
+    for (int e = 0; e < 16; ++e) sum += v[e];
+  }
+  for (; k + 4 <= n; k += 4) {
+    f32x4 v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const f32x4*>(s + (k + e) * step);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += v[e];
   }
   for (; k < n; ++k) sum += *reinterpret_cast<const f32x4*>(s + k * step);
   return sum;
@@ -412,10 +419,11 @@ struct ReduceArgs {
   int dx_strips, dx_c, c4, dx_vec;
   unsigned dw_blocks;
 };
+static constexpr int kReduce = 64;      // threads: a small dW still spreads over the card
 template <typename T>
-__global__ __launch_bounds__(256) void gate_reduce_kernel(ReduceArgs a) {
+__global__ __launch_bounds__(kReduce) void gate_reduce_kernel(ReduceArgs a) {
   if (blockIdx.x >= a.dw_blocks) {
-    const int64_t i = (int64_t)(blockIdx.x - a.dw_blocks) * 256 + threadIdx.x, m = i / (a.c4 / 4);
+    const int64_t i = (int64_t)(blockIdx.x - a.dw_blocks) * kReduce + threadIdx.x, m = i / (a.c4 / 4);
     const int c = (int)(i - m * (a.c4 / 4)) * 4;
     if (m >= a.rows) return;
     const f32x4 v = ordered_sum(a.dx_part + m * a.c4 + c, a.dx_strips, a.rows * a.c4);
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(256) void gate_reduce_kernel(ReduceArgs a) {
     store4<T>(static_cast<T*>(a.dx) + m * a.dx_ld + c, o, a.dx_c - c, a.dx_vec);
     return;
   }
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * kReduce + threadIdx.x;
   const int quads = a.fp / 2;
   const int64_t ci = i / quads;
   const int p = (int)(i - ci * quads) * 4;
@@ -856,9 +864,9 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
     b.part = part; b.db = a.db; b.dwg = dwg; b.dwu = dwu; b.dbg = dbg; b.dbu = dbu; b.c = dw ? d->c : 0;
     b.strips = p.strips; b.db_tiles = p.db_tiles; b.f = d->f; b.fp = p.fp; b.bf = bf;
     b.dx_part = dxp; b.dx = dx; b.rows = d->rows; b.dx_ld = d->x_ld; b.dx_strips = p.dx_strips; b.dx_c = d->c; b.c4 = p.c4; b.dx_vec = dx_vec;
-    b.dw_blocks = (unsigned)ceil_div64((b.c + (a.db ? 1 : 0)) * (p.fp / 2), 256);
-    const unsigned dx_blocks = dxp ? (unsigned)ceil_div64(d->rows * (p.c4 / 4), 256) : 0;
-    hipLaunchKernelGGL((gate_reduce_kernel<T>), dim3(b.dw_blocks + dx_blocks), dim3(256), 0, st, b);
+    b.dw_blocks = (unsigned)ceil_div64((b.c + (a.db ? 1 : 0)) * (p.fp / 2), kReduce);
+    const unsigned dx_blocks = dxp ? (unsigned)ceil_div64(d->rows * (p.c4 / 4), kReduce) : 0;
+    hipLaunchKernelGGL((gate_reduce_kernel<T>), dim3(b.dw_blocks + dx_blocks), dim3(kReduce), 0, st, b);
     SSMI_LAUNCH_CHECK();
   }
   return SSMI_OK;
