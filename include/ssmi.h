@@ -801,7 +801,7 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
  * sums of the unrounded ones.
  * Results are the same on every call (no atomics).  x, w_gate, w_up and ws 16-byte aligned; at most 65536 channels and units and
  * 2^31 - 1 rows, tensors may pass 2 GiB.  ws: ssmi_gated_ff_workspace_bytes(d, backward) (0 = none; 0 for a refused descriptor too).
- * Up to 16 rows are answered by a kernel that only streams the kernels.  No counterpart in the reference. */
+ * A few rows are answered by a kernel that only streams the parameters.  No counterpart in the reference. */
 enum { SSMI_GATE_SWISH = 0, SSMI_GATE_GELU = 1, SSMI_GATE_RELU = 2, SSMI_GATE_SIGMOID = 3 };
 typedef struct ssmi_gated_desc {
   int64_t rows, x_ld, y_ld;

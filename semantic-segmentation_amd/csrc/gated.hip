@@ -793,12 +793,17 @@ static ssmi_status launch_rows(const GateArgs& a, hipStream_t st) {
   return SSMI_OK;
 }
 
-// Rows that gate_rows_kernel takes: as many as it beats the tiles at.  Its and their times in us, bfloat16: 1 x 512 -> 2048 3.9 and 5.9, 2 rows
-// 4.7 and 5.9, 4 rows 6.1 and 5.9, 1 x 2048 -> 4096 14 and 19.  Under float32 parameters the tiles need a bfloat16 copy of them first (1 x 512
-// -> 2048 4.2 and 12.5, 16 rows 8.7 and 12.5), and in float32 they cannot hide a long reduction (1 row 4.0 and 20, 24 rows 9.8 and 20.6,
-// 48 rows 17 and 21).  Its rows of x have to fit LDS: eight of 2048 float32.
+// Rows that gate_rows_kernel takes: as many as it beats the tiles at.  Its and their times in us:
+//   bfloat16                        1 x 512 -> 2048 3.9 and 5.9, 2 rows 4.7 and 5.9, 4 rows 6.1 and 5.9, 1 x 2048 -> 4096 14 and 19
+//   bfloat16, float32 parameters    1 x 512 -> 2048 4.2 and 12.5, 16 rows 8.7 and 12.5: the tiles need a bfloat16 copy of the parameters;
+//                                   4 x 96 -> 301 5.9 and 6.3, 8 rows 8.0 and 6.5
+//   float32                         1 x 512 -> 2048 4.0 and 20, 24 rows 9.8 and 20.6, 48 rows 17 and 21: few tiles cannot hide a long reduction;
+//                                   16 x 96 -> 301 7.6 and 8.7
+// Its rows of x have to fit LDS: eight of 2048 float32.
 static bool takes_rows_kernel(const ssmi_gated_desc* d) {
-  return d->rows <= (d->param_dtype == SSMI_BF16 ? 2 : d->dtype == SSMI_BF16 ? 16 : 32) && d->c <= 2048;
+  const bool long_c = d->c >= 256;
+  const int most = d->param_dtype == SSMI_BF16 ? 2 : d->dtype == SSMI_BF16 ? (long_c ? 16 : 4) : (long_c ? 32 : 16);
+  return d->rows <= most && d->c <= 2048;
 }
 
 template <typename T>

@@ -114,10 +114,10 @@ def test_forward(rows, c, f, dtype, pdtype):
 
 
 @pytest.mark.parametrize("dtype,pdtype", TYPES)
-@pytest.mark.parametrize("c,f", [(48, 64), (20, 36), (7, 33), (2048, 40), (2049, 40)])
+@pytest.mark.parametrize("c,f", [(48, 64), (20, 36), (7, 33), (255, 40), (256, 40), (2048, 40), (2049, 40)])
 def test_every_count_of_few_rows(c, f, dtype, pdtype):
     """The borders between the kernel of few rows (1, 2, 4 or 8 at a time) and the tiles; more channels than it takes."""
-    for rows in (1, 2, 3, 4, 7, 8, 9, 15, 16, 17, 31, 32, 33):
+    for rows in (1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 32, 33):
         x, ws, bs, _ = make(rows, c, f, dtype, pdtype, rows % 2 == 1, rows + c + f)
         y, err, _, _ = reference(x, ws, bs, None, "swish", dtype)
         got = ff.gated_feed_forward(x.to(DEV), *(w.to(DEV) for w in ws), *(None if b is None else b.to(DEV) for b in bs), activation="swish")
