@@ -66,14 +66,14 @@ def quantize_mx4_weights(w: torch.Tensor) -> MX4Weights:
     return MX4Weights(codes, scales, k)
 
 
-def _operand(x, w: MX4Weights, who):
+def _operand(x, w: MX4Weights, who, *biases):
     require_gpu(x, who)
     if not isinstance(w, MX4Weights):
         raise TypeError("{}: MX4Weights expected, got {}".format(who, type(w).__name__))
     if x.dim() < 1 or x.shape[-1] != w.k or w.codes.device != x.device:
         raise ValueError("{}: x [..., {}] on {} expected, got {} on {}".format(who, w.k, w.codes.device, tuple(x.shape), x.device))
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise ValueError("{}: 4-bit products have no backward pass; call them under torch.no_grad() or on a detached input".format(who))
+    if torch.is_grad_enabled() and (x.requires_grad or any(isinstance(b, torch.Tensor) and b.requires_grad for b in biases)):
+        raise ValueError("{}: 4-bit products have no backward pass; call them under torch.no_grad() or on detached tensors".format(who))
     t, rows, ld = rows_of(x)
     return t, rows, ld, torch.empty(x.shape[:-1] + (w.n,), dtype=x.dtype, device=x.device)
 
@@ -91,7 +91,7 @@ def _workspace(rows, k, like):
 def mx4_dense(x: torch.Tensor, w: MX4Weights, bias=None) -> torch.Tensor:
     """q(x) w + bias: x [..., k] float32 or bfloat16, the result in x's type; bias float32 [n] or None."""
     who = "mx4_dense"
-    t, rows, ld, y = _operand(x, w, who)
+    t, rows, ld, y = _operand(x, w, who, bias)
     code = dtype_code(x, who)
     bias = vector(bias, w.n, x, who, "bias", optional=True)
     if rows:
@@ -105,7 +105,7 @@ def mx4_dense(x: torch.Tensor, w: MX4Weights, bias=None) -> torch.Tensor:
 def mx4_gated(x, w_gate, w_up, b_gate, b_up, activation):
     """layers.feed_forward.gated_feed_forward on 4-bit weights."""
     who = "gated_feed_forward"
-    t, rows, ld, y = _operand(x, w_gate, who)
+    t, rows, ld, y = _operand(x, w_gate, who, b_gate, b_up)
     if not isinstance(w_up, MX4Weights) or (w_up.k, w_up.n) != (w_gate.k, w_gate.n) or w_up.codes.device != x.device:
         raise ValueError("{}: two MX4Weights of one shape on {} expected".format(who, x.device))
     code = dtype_code(x, who)

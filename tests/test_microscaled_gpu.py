@@ -257,3 +257,15 @@ def test_exponents_of_other_programs():
     want = (v.reshape(5, 2, 32) * torch.ldexp(torch.ones(5, 2, dtype=torch.float64), scales.int() - 127)[..., None]).reshape(5, 64).t()
     over = want.abs() > torch.finfo(torch.float32).max
     assert torch.equal(w[~over], want[~over]) and bool(torch.isinf(w[over]).all())
+
+
+def test_biases_that_ask_for_gradients_are_refused():
+    x = data(3, 40, torch.float32, 1).to(DEV)
+    q = [ms.quantize_mx4_weights(data(40, 8, torch.float32, s).to(DEV)) for s in (2, 3)]
+    b = torch.zeros(8, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError):
+        ms.mx4_dense(x, q[0], b)
+    with pytest.raises(ValueError):
+        ff.gated_feed_forward(x, *q, b.detach(), b)
+    with torch.no_grad():
+        assert torch.equal(ms.mx4_dense(x, q[0], b), ms.mx4_dense(x, q[0]))
