@@ -576,18 +576,20 @@ static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
 //   gate: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
-//   dx:   256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192; 64 x 64 where 128 x 64
+//   no tile of 128 rows or channels where there are 64 (131k x 64 -> 256 float32, dx 142 -> 103 us, dW 127 -> 90)
+//   dx:   256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192; 64 x 64 under 64 channels or where 128 x 64
 //         makes under 384 (4096 x 512 -> 2048 bfloat16 41 -> 36 us, 16k x 128 -> 512 float32 49 -> 47); else as above
 //   dW:   128 x 256 under strips of 4096 rows; else as above, counting the strips
 // float32 takes no wide tiles: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
 enum Tile { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 static Tile tile_for(int64_t q, int64_t p, bool wide, int64_t times = 1) {
   if (wide && ceil_div64(q, 256) * ceil_div64(p, 128) * times >= 384 && q > 128) return kTile128x256;
-  return ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
+  return q > 64 && ceil_div64(q, 128) * ceil_div64(p, 128) * times >= 256 ? kTile128x128 : kTile128x64;
 }
 static Tile tile_for_dx(int64_t rows, int64_t c, bool wide) {
   if (wide && c > 128 && ceil_div64(rows, 256) * ceil_div64(c, 256) >= 192) return kTile256x256;
   const Tile t = tile_for(rows, c, false);
+  if (c <= 64) return kTile64x64;
   return t == kTile128x64 && ceil_div64(rows, 64) * ceil_div64(c, 128) < 384 ? kTile64x64 : t;
 }
 static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t most_strips) {
@@ -595,13 +597,24 @@ static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t m
   if (wide && c > 128 && rows / ceil_div64(512, ceil_div64(p, 128) * ceil_div64(c, 256)) >= 4096) return kTile128x256;
   return tile_for(c, p, false, most_strips);
 }
-// K steps that a strip of dx takes: all of them, unless its smallest tiles leave half of the card idle; then two workgroups to a CU, each with
-// 256 bfloat16 or 128 float32 values at least.  Whole backward pass, one strip and so: 64 x 64 -> 4096 bfloat16 122 and 20 us, float32 205
-// and 25; 31 x 80 -> 944 42 and 17, 60 and 22; strips of four times as many values 23, 31, 23 and 31.
-static int dx_each(Tile t, int64_t rows, int64_t c, int steps) {
+// K steps that a strip of dx takes.  Its smallest tiles may leave the card idle under a long K; strips bring one or two workgroups to a CU, of
+// four steps (256 bfloat16, 128 float32 values) at least.  By measurement a step takes a workgroup 0.4 us in bfloat16, two workgroups of a CU
+// side by side, and 0.85 in float32, where the matrix unit is full with one of them; the strips' sums and their reduction take 6.
+// Whole backward pass, one strip and so: 64 x 64 -> 4096 bfloat16 122 and 20 us, float32 205 and 25; 31 x 80 -> 944 42 and 17, 60 and 21;
+// dx alone, one strip and two, where they do not pay: 16k x 64 -> 256 bfloat16 6.5 and 14, 2048 x 512 -> 512 8.5 and 15, float32 17 and 20, 27 and 29.
+static int dx_each(Tile t, int64_t rows, int64_t c, int steps, bool bf) {
   const int64_t tiles = ceil_div64(rows, 64) * ceil_div64(c, 64);
-  if (t != kTile64x64 || tiles > 256) return steps;
-  return (int)std::max<int64_t>(ceil_div64(steps, 512 / tiles), 512 / 128);      // steps of 128 bytes
+  int best = steps;
+  if (t != kTile64x64 || tiles > 256) return best;
+  const int64_t step_ns = bf ? 400 : 850, strips_ns = 6000;
+  int64_t least = steps * step_ns;
+  for (int per_cu = 1; per_cu <= 2; ++per_cu) {
+    const int64_t strips = 256 * per_cu / tiles;
+    if (strips < 2) continue;
+    const int64_t each = std::max<int64_t>(ceil_div64(steps, strips), 4), ns = each * step_ns * (bf ? 1 : per_cu) + strips_ns;
+    if (ns < least) { least = ns; best = (int)each; }
+  }
+  return best;
 }
 static inline int64_t q_side(Tile t) { return t <= kTile128x64 ? 64 : t == kTile128x128 ? 128 : 256; }
 
@@ -652,7 +665,7 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
   p.c4 = (int)up_to(d->c, 4);
   const int steps = (p.split ? 4 : 2) * (int)ceil_div64(p.fp * p.es, ProductShape<1, 1>::kStep);
-  p.dx_each = dx_each(p.dx_tile, d->rows, d->c, steps);
+  p.dx_each = dx_each(p.dx_tile, d->rows, d->c, steps, bf);
   p.dx_strips = (int)ceil_div64(steps, p.dx_each);
   p.dx_bytes = p.dx_strips > 1 ? up256((size_t)p.dx_strips * d->rows * p.c4 * 4) : 0;
   p.db_tiles = (int)ceil_div64(d->rows, q_side(p.gate_tile));
