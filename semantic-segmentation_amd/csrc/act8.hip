@@ -37,15 +37,19 @@ __device__ __forceinline__ void load_piece(const T* p, int n, float (&v)[N]) {
     for (int i = 0; i < N; ++i) v[i] = i < n ? Act<T>::gld(p + i) : 0.f;
   }
 }
-template <typename T, bool VEC, int N>
+// PAST: past the caches
+template <typename T, bool VEC, bool PAST, int N>
 __device__ __forceinline__ void store_piece(T* p, int n, const float (&v)[N]) {
   if constexpr (VEC) {
+    u32x4 w;
     if constexpr (sizeof(T) == 2) {
       const u32x2 x = pack_bf16x4(f32x4{v[0], v[1], v[2], v[3]}), y = pack_bf16x4(f32x4{v[4], v[5], v[6], v[7]});
-      *reinterpret_cast<u32x4*>(p) = u32x4{x[0], x[1], y[0], y[1]};
+      w = u32x4{x[0], x[1], y[0], y[1]};
     } else {
-      Act<T>::gst4(p, f32x4{v[0], v[1], v[2], v[3]});
+      w = __builtin_bit_cast(u32x4, (f32x4{v[0], v[1], v[2], v[3]}));
     }
+    if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+    else *reinterpret_cast<u32x4*>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -174,7 +178,7 @@ __device__ __forceinline__ void decode(const unsigned (&w)[N / 4], unsigned byte
 
 // BN: also the output of the BatchNormalization -> activation -> SpatialDropout behind the stored tensor, which the backward pass
 // needs beside it (operand of the next weight gradient); y (nullable) the restored tensor itself
-template <typename T, bool VEC, bool BN>
+template <typename T, bool VEC, bool BN, bool PAST>
 __global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t npix, int c,
                                                            int groups, T* __restrict__ y, int64_t ld_y, RestoreBn bn, T* __restrict__ out,
                                                            int64_t ld_out) {
@@ -207,7 +211,7 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __rest
       if (px >= npix) break;
       float v[N];
       decode<N>(w[s], sc[s], v);
-      if (!BN || y) store_piece<T, VEC>(y + px * ld_y + l.ch, l.n, v);
+      if (!BN || y) store_piece<T, VEC, PAST>(y + px * ld_y + l.ch, l.n, v);
       if constexpr (BN) {
         float drop[N];
 #pragma unroll
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const uint8_t* __rest
           const float r = z > 0.f ? z : slope[i] * z;
           v[i] = r * drop[i];
         }
-        store_piece<T, VEC>(out + px * ld_out + l.ch, l.n, v);
+        store_piece<T, VEC, PAST>(out + px * ld_out + l.ch, l.n, v);
       }
     }
   }
@@ -281,8 +285,8 @@ ssmi_status ssmi_act8_restore(const uint8_t* codes, const uint8_t* scales, int64
     const bool vec = c % 8 == 0 && ld_y % 8 == 0 && aligned16(y) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
     T* yt = static_cast<T*>(y);
     const RestoreBn none = {};
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, false, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, false, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, none, (T*)nullptr, (int64_t)0);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });
@@ -304,9 +308,14 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
   return dispatch_dtype(dtype, [&](auto tag) -> ssmi_status {
     using T = decltype(tag);
     const bool vec = c % 8 == 0 && ld_out % 8 == 0 && aligned16(out) && (!y || (ld_y % 8 == 0 && aligned16(y))) && (!drop || aligned16(drop)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
+    // Two results of 256 MB and more together do not stay in the memory-side cache of that size; written past the caches they take 115 us
+    // instead of 131 (1M x 64 float32), with a reader behind them 264 instead of 284.  Under it the reader is faster with them there (2 x 67 MB
+    // 73 us, past the caches 75); one result of any size measures the same either way.
+    const bool past = npix * c * (int64_t)sizeof(T) * (y ? 2 : 1) >= (256ll << 20);
     T *yt = static_cast<T*>(y), *ot = static_cast<T*>(out);
-    if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    if (vec && past) hipLaunchKernelGGL((act8_restore_kernel<T, true, true, true>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    else if (vec) hipLaunchKernelGGL((act8_restore_kernel<T, true, true, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, false, true, false>), blocks_for<T>(npix, groups), dim3(256), 0, as_stream(stream), codes, scales, npix, c, groups, yt, ld_y, p, ot, ld_out);
     SSMI_LAUNCH_CHECK();
     return SSMI_OK;
   });

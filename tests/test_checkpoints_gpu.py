@@ -158,3 +158,15 @@ def test_more_groups_than_a_block_holds(c):
     x = _data(37, c, torch.float32, c).to(DEV)
     _check(x, cp.store_8bit(x))
     _check(x.bfloat16(), cp.store_8bit(x.bfloat16()))
+
+
+@pytest.mark.parametrize("dtype,px", [(torch.float32, 1100 * 1000), (torch.bfloat16, 2200 * 1000)])
+def test_results_larger_than_the_caches_are_those_of_their_halves(dtype, px):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(px, 32, generator=g, device=DEV).to(dtype)
+    bn = [torch.rand(32, generator=g, device=DEV) + 0.5 for _ in range(4)]
+    y, out = cp.store_8bit(x).restore_bn_act(*bn, activation="leaky")
+    assert 2 * y.numel() * y.element_size() >= 256 << 20
+    for part in (slice(0, px // 2), slice(px // 2, px)):
+        ys, outs = cp.store_8bit(x[part]).restore_bn_act(*bn, activation="leaky")
+        assert torch.equal(y[part], ys) and torch.equal(out[part], outs)
