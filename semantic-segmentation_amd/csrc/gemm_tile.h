@@ -294,16 +294,19 @@ struct TileRows {
   }
 };
 
-// four values to memory, bfloat16 with one conversion per pair
-template <typename T>
+// four values to memory, bfloat16 with one conversion per pair; PAST: past the caches
+template <typename T, bool PAST = false>
 __device__ __forceinline__ void put4(T* p, f32x4 v) {
   if constexpr (sizeof(T) == 2) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     const bf16x2 a = __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2), b = __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2);
-    *reinterpret_cast<u32x2*>(p) = u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    const u32x2 w = {__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<u32x2*>(p));
+    else *reinterpret_cast<u32x2*>(p) = w;
   } else {
-    *reinterpret_cast<f32x4*>(p) = v;
+    if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p));
+    else *reinterpret_cast<f32x4*>(p) = v;
   }
 }
 

@@ -123,7 +123,7 @@ struct Mx4Args {
   const float* bias[2];
   void* y;
   int64_t rows, y_ld;
-  int n, nb, act, vec_out;
+  int n, nb, act, vec_out, past;
   unsigned np, nq;
 };
 
@@ -305,7 +305,10 @@ __global__ __launch_bounds__(256, 2) void mx4_kernel(Mx4Args a) {
       }
       return o;
     };
-    if (whole) {
+    if (whole && a.past) {
+      R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), wq, pos, [](int) {},
+                                  [&](const float* row, int qc, int) __attribute__((always_inline)) { put4<T, true>(y + qc * a.y_ld + lane_at, value(row)); });
+    } else if (whole) {
       R::template run<R::kRounds>(acc, reinterpret_cast<float*>(smem), wq, pos, [](int) {},
                                   [&](const float* row, int qc, int) __attribute__((always_inline)) { put4<T>(y + qc * a.y_ld + lane_at, value(row)); });
     } else {
@@ -475,6 +478,9 @@ static ssmi_status mx4_product(const char* who, const void* x, int64_t x_ld, int
     a.xc = codes;
     a.xs = scales;
     a.vec_out = a.y_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & (4 * sizeof(T) - 1)) == 0;
+    // Results of 128 MB and more go past the caches: 64k x 512 -> 1024 float32 78 us, through them 97, with a reader behind it 173 and 193;
+    // 32k rows 42 and 42, 85 and 90.  Under that the reader finds them there: 16k rows 24 and 25, 45.6 and 43.7.
+    a.past = rows * n * (int64_t)sizeof(T) >= (128ll << 20);
     return launch_tiles<T, 2, 2, GATE>(a, as_stream(stream));
   });
 }

@@ -269,3 +269,13 @@ def test_biases_that_ask_for_gradients_are_refused():
         ff.gated_feed_forward(x, *q, b.detach(), b)
     with torch.no_grad():
         assert torch.equal(ms.mx4_dense(x, q[0], b), ms.mx4_dense(x, q[0]))
+
+
+@pytest.mark.parametrize("dtype,rows,n", [(torch.float32, 34000, 1000), (torch.bfloat16, 70001, 1028)])
+def test_results_larger_than_the_caches_are_those_of_their_parts(dtype, rows, n):
+    x = data(rows, 64, dtype, 5).to(DEV)
+    q = [ms.quantize_mx4_weights(data(64, n, torch.float32, s).to(DEV) / 8) for s in (1, 2)]
+    y, z = ms.mx4_dense(x, q[0]), ff.gated_feed_forward(x, *q)
+    assert y.numel() * y.element_size() >= 128 << 20
+    for part in (slice(0, 2000), slice(rows - 2000, rows)):
+        assert torch.equal(y[part], ms.mx4_dense(x[part], q[0])) and torch.equal(z[part], ff.gated_feed_forward(x[part], *q))
