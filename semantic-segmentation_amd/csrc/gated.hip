@@ -4,7 +4,7 @@
 // happen in registers and g, u never reach memory.
 // Backward: nothing but x is kept.  One kernel recomputes g and u (exact float32 in registers, where storing them would round them to
 // the activation type or double the traffic) and forms in its epilogue, from dy,
-//   dg = dy * u * act'(g),   du = dy * act(g)                              one row [dg | du] per pixel, activation type
+//   dg = dy * u * act'(g),   du = dy * act(g)                              one row [dg | du] per pixel, float32 or two bfloat16 terms
 // then  dx = dg Wg^T + du Wu^T  (one product over 2 f) and  dW = x^T dg, x^T du  (one product over the rows, split into strips whose
 // float32 partial sums are added in a fixed order: results do not depend on the launch).
 // All products run on gemm_tile.h: bfloat16 32x32x16 or float32 32x32x2 matrix instructions, float32 sums throughout.
@@ -43,10 +43,15 @@ struct GateArgs {
   int64_t rows, x_ld, w_ld, out_ld, dy_ld;
   int c, f, fp;                 // fp: units with the padding that [dg | du] rows have
   int act, bf_params, vec_out, vec_dy;      // see vec_of
-  int split;                    // backward: [dg | du] as two bfloat16 terms each, [dg | du | rest of dg | rest of du]
   float* db;                    // backward: column sums of [dg | du] per row tile, or nullptr
   unsigned np, nq;
 };
+
+// Columns of the projections' gradients, in units of fp: float32 [dg | du], bfloat16 [dg | du | rest of dg | rest of du].  One bfloat16 of
+// dg is off by up to 2^-8 of it and shows beside the results' own rounding (bfloat16 results of 9999 x 256 -> 682 off by 2.3e-3 of their norm
+// instead of the 1.7e-3 of that rounding, float32 ones by 1.7e-3); the second term brings it to 2^-16 (1.7e-3 and 2.5e-6) for twice the
+// arithmetic of dx and dW (64k x 512 -> 2048: with dg and du 420 -> 490 us, dx 233 -> 469, dW 253 -> 514).
+template <typename T> constexpr int kGradSides = sizeof(T) == 2 ? 4 : 2;
 
 template <typename T, int SP, int SQ>
 struct GateSides : GateShape<SP, SQ> {
@@ -111,14 +116,14 @@ __global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(
   const T* const dyt = static_cast<const T*>(a.dy) + (BWD ? m0 * a.dy_ld + f0 : 0);
   const unsigned o_lane = (unsigned)R::first() * (unsigned)a.out_ld + (unsigned)col, d_lane = (unsigned)R::first() * (unsigned)a.dy_ld + (unsigned)col;
   float sum[BWD ? 8 : 1] = {};
-  // [dg | du] of four units of a pixel; with `split` the parts that bfloat16 leaves behind follow
+  // [dg | du] of four units of a pixel; behind them the parts that bfloat16 leaves
   auto put_gradients = [&](T* d, const float (&o)[4], const float (&v)[4]) __attribute__((always_inline)) {
     if constexpr (BWD) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) { sum[e] += o[e]; sum[4 + e] += v[e]; }
       put4<T>(d, f32x4{o[0], o[1], o[2], o[3]});
       put4<T>(d + a.fp, f32x4{v[0], v[1], v[2], v[3]});
-      if (sizeof(T) == 2 && SQ < 4 && a.split) {      // problems this small take the smaller tiles
+      if constexpr (sizeof(T) == 2) {
         f32x4 ro, rv;
 #pragma unroll
         for (int e = 0; e < 4; ++e) { ro[e] = o[e] - (float)(T)o[e]; rv[e] = v[e] - (float)(T)v[e]; }
@@ -243,14 +248,14 @@ __global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(
 }
 
 // dx[m][c] = sum_f dg[m][f] Wg[c][f] + du[m][f] Wu[c][f]: K runs over the units of the first, then of the second projection (and again
-// over the second terms of a split [dg | du]).  Few tiles under a long K share it in strips, whose float32 sums [strip][rows][c4] are added
+// over the second terms of bfloat16).  Few tiles under a long K share it in strips, whose float32 sums [strip][rows][c4] are added
 // in their order by the reduction behind dW.
 struct GateDxArgs {
   const void *dgu, *wg, *wu;
   void* dx;
   float* part;      // more than one strip: instead of dx
   int64_t rows, w_ld, dx_ld;
-  int c, fp, vec_out, sides;      // sides: 2, or 4 when split
+  int c, fp, vec_out;
   int each, strips, c4;           // K steps of a strip
   unsigned np, nq;
 };
@@ -293,12 +298,12 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_k
   s.fp = a.fp;
   s.half = (a.fp + S::W::kStepK - 1) / S::W::kStepK;
   s.first = (int)strip * a.each;
-  s.end = min(s.first + a.each, a.sides * s.half);
+  s.end = min(s.first + a.each, kGradSides<T> * s.half);
   s.wp = wave >> 1;
   s.wq = wave & 1;
   s.wg.init(static_cast<const T*>(a.wg) + c0 * a.w_ld, a.w_ld, a.c - c0);
   s.wu = make_rsrc(static_cast<const T*>(a.wu) + c0 * a.w_ld, 0x7FFFFFFFu);
-  s.d.init(static_cast<const T*>(a.dgu) + m0 * (a.sides * (int64_t)a.fp), a.sides * (int64_t)a.fp, (int)min((int64_t)(SQ * 64), a.rows - m0));
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (kGradSides<T> * (int64_t)a.fp), kGradSides<T> * (int64_t)a.fp, (int)min((int64_t)(SQ * 64), a.rows - m0));
   s.rw.init(lane);
   s.rd.init(lane);
   f32x16 acc[SP][SQ];
@@ -328,12 +333,12 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dx_k
   }
 }
 
-// part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]; a split [dg | du] goes through the rows twice
+// part[strip][c][2 fp] = sum over the strip's rows of x[m][c] [dg | du][m][p]; bfloat16 goes through the rows twice, the second time with the second terms
 struct GateDwArgs {
   const void *x, *dgu;
   float* part;
   int64_t rows, x_ld, strip_rows;
-  int c, cp, fp, sides;         // cp: channels with the padding of x rows
+  int c, cp, fp;                // cp: channels with the padding of x rows
   unsigned np, nq;
 };
 template <typename T, int SP, int SQ>
@@ -370,9 +375,9 @@ __global__ __launch_bounds__(256, (ProductShape<SP, SQ>::kPerCu)) void gate_dw_k
   s.rows = (int)min(a.strip_rows, a.rows - m0);
   s.wp = wave >> 1;
   s.wq = wave & 1;
-  s.d.init(static_cast<const T*>(a.dgu) + m0 * (a.sides * (int64_t)a.fp) + p0, a.sides * (int64_t)a.fp, 2 * a.fp - p0);
+  s.d.init(static_cast<const T*>(a.dgu) + m0 * (kGradSides<T> * (int64_t)a.fp) + p0, kGradSides<T> * (int64_t)a.fp, 2 * a.fp - p0);
   s.once = (s.rows + S::D::kStepK - 1) / S::D::kStepK;
-  s.times = a.sides / 2;
+  s.times = kGradSides<T> / 2;
   s.second = 2u * (unsigned)a.fp * (unsigned)sizeof(T);
   s.x.init(static_cast<const T*>(a.x) + m0 * a.x_ld + c0, a.x_ld, a.cp - c0);
   s.rd.init(lane);
@@ -625,7 +630,6 @@ struct GatePlan {
   Tile gate_tile, dx_tile, dw_tile;
   int strips;
   int64_t strip_rows;
-  bool split;                       // [dg | du] in two bfloat16 terms
   int db_tiles;
   int dx_each, dx_strips, c4;
   size_t w_bytes, x_bytes, dgu_bytes, part_bytes, db_bytes, dx_bytes;
@@ -644,12 +648,9 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   p.pad_x = p.cp != d->c || d->x_ld % p.ce != 0;
   p.w_bytes = p.pad_w ? 2 * up256((size_t)d->c * p.fp * p.es) : 0;
   p.x_bytes = p.pad_x ? up256((size_t)d->rows * p.cp * p.es) : 0;
-  // One bfloat16 of dg and du is off by up to 2^-9 and shows beside the output's own rounding; two are exact to 2^-17 and cost the two
-  // products that read them twice the arithmetic: some ten us up to 2^27 multiplications (the backward pass of 102 x 893 -> 391: 35 us with
-  // one term, 43 with two; 512 x 512 -> 512: 26 and 38), too much above (4096 x 256 -> 1024: 48 and 72; 16k x 512 -> 2048: 247 and 440).
-  p.split = bf && (double)d->rows * d->c * d->f <= (double)(1 << 27);
-  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, bf && !p.split);      // the wide tile's epilogue has no registers for the second terms
-  p.dgu_bytes = up256((size_t)d->rows * (p.split ? 4 : 2) * p.fp * p.es);
+  const int sides = bf ? kGradSides<bf16> : kGradSides<float>;
+  p.gate_tile = tile_for(d->rows, 2 * (int64_t)d->f, bf);
+  p.dgu_bytes = up256((size_t)d->rows * sides * p.fp * p.es);
   // strips of the weight gradient: one round of workgroups (two to a CU), each strip long enough to be worth its partial sums (512 rows)
   // and, in float32, short enough for the running sums (4096 rows: 2^-24 sqrt(4096) of a term)
   const int64_t most = ceil_div64(d->rows, 512), least = bf ? 1 : ceil_div64(d->rows, 4096);
@@ -658,13 +659,13 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   strips = strips < most ? strips : most;
   strips = strips > least ? strips : least;
   // a strip is addressed with 32-bit offsets from its first row: under 2^31 - 2^27 bytes of [dg | du] and of x
-  const int64_t row_bytes = p.es * std::max<int64_t>((p.split ? 4 : 2) * (int64_t)p.fp, p.pad_x ? p.cp : d->x_ld);
+  const int64_t row_bytes = p.es * std::max<int64_t>(sides * (int64_t)p.fp, p.pad_x ? p.cp : d->x_ld);
   const int64_t reach = std::max<int64_t>(((1ll << 31) - (1ll << 27)) / row_bytes / 64 * 64, 64);
   p.strip_rows = std::min(up_to(ceil_div64(d->rows, strips), 64), reach);
   p.strips = (int)ceil_div64(d->rows, p.strip_rows);
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
   p.c4 = (int)up_to(d->c, 4);
-  const int steps = (p.split ? 4 : 2) * (int)ceil_div64(p.fp * p.es, ProductShape<1, 1>::kStep);
+  const int steps = sides * (int)ceil_div64(p.fp * p.es, ProductShape<1, 1>::kStep);
   p.dx_each = dx_each(p.dx_tile, d->rows, d->c, steps, bf);
   p.dx_strips = (int)ceil_div64(steps, p.dx_each);
   p.dx_bytes = p.dx_strips > 1 ? up256((size_t)p.dx_strips * d->rows * p.c4 * 4) : 0;
@@ -853,9 +854,8 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   GateArgs a = {};
   a.x = s.x; a.wg = s.wg; a.wu = s.wu; a.bg = bg; a.bu = bu; a.dy = dy; a.out = dgu;
   SSMI_LAUNCH_CHECK();
-  const int sides = p.split ? 4 : 2;
-  a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = sides * (int64_t)p.fp; a.dy_ld = d->y_ld;
-  a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf; a.split = p.split;
+  a.rows = d->rows; a.x_ld = s.x_ld; a.w_ld = s.w_ld; a.out_ld = kGradSides<T> * (int64_t)p.fp; a.dy_ld = d->y_ld;
+  a.c = d->c; a.f = d->f; a.fp = p.fp; a.act = d->act; a.bf_params = bf;
   a.db = dbg || dbu ? dbp : nullptr;
   a.vec_out = 2;      // rows of whole 16 bytes
   a.vec_dy = vec_of(d->y_ld, dy, p.es);
@@ -865,7 +865,7 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   if (dx) {
     GateDxArgs b = {};
     b.part = dxp; b.each = p.dx_each; b.strips = p.dx_strips; b.c4 = p.c4;
-    b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp; b.sides = sides;
+    b.dgu = dgu; b.wg = s.wg; b.wu = s.wu; b.dx = dx; b.rows = d->rows; b.w_ld = s.w_ld; b.dx_ld = d->x_ld; b.c = d->c; b.fp = p.fp;
     b.vec_out = dx_vec;
     r = launch_dx<T>(p.dx_tile, b, st);
     if (r != SSMI_OK) return r;
@@ -873,7 +873,7 @@ static ssmi_status gated_bwd(const ssmi_gated_desc* d, const void* x, const void
   const bool dw = dwg || dwu;
   if (dw) {
     GateDwArgs b = {};
-    b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp; b.sides = sides;
+    b.x = s.x; b.dgu = dgu; b.part = part; b.rows = d->rows; b.x_ld = s.x_ld; b.strip_rows = p.strip_rows; b.c = d->c; b.cp = p.cp; b.fp = p.fp;
     r = launch_dw<T>(p.dw_tile, b, p.strips, st);
     if (r != SSMI_OK) return r;
   }
