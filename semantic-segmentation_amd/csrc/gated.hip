@@ -53,6 +53,12 @@ struct GateArgs {
 // arithmetic of dx and dW (64k x 512 -> 2048: with dg and du 420 -> 490 us, dx 233 -> 469, dW 253 -> 514).
 template <typename T> constexpr int kGradSides = sizeof(T) == 2 ? 4 : 2;
 
+// what the first bfloat16 term leaves; an infinity leaves nothing (inf - inf would turn it into a NaN), a NaN is one in the first term already
+__device__ __forceinline__ float rest_of(float v) {
+  const float first = (float)(bf16)v;
+  return __builtin_fabsf(first) < INFINITY ? v - first : 0.f;
+}
+
 template <typename T, int SP, int SQ>
 struct GateSides : GateShape<SP, SQ> {
   using GateShape<SP, SQ>::kStep;
@@ -126,7 +132,7 @@ __global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(
       if constexpr (sizeof(T) == 2) {
         f32x4 ro, rv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { ro[e] = o[e] - (float)(T)o[e]; rv[e] = v[e] - (float)(T)v[e]; }
+        for (int e = 0; e < 4; ++e) { ro[e] = rest_of(o[e]); rv[e] = rest_of(v[e]); }
         put4<T>(d + 2 * a.fp, ro);
         put4<T>(d + 3 * a.fp, rv);
       }

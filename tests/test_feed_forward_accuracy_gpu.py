@@ -50,3 +50,17 @@ def test_bfloat16_gradients_are_as_exact_as_their_type(rows, c, f, pdtype):
         else:
             r = off(a, b.to(torch.bfloat16).double())
             assert r <= 2.0 ** -11, (name, r)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,c,f", [(9, 40, 21), (150, 72, 64), (2100, 256, 264)])
+def test_an_infinite_gradient_stays_infinite(rows, c, f, dtype):
+    """One infinite value of dy: its row of dx and its columns of the kernels' gradients are the infinities (or, where two of them meet, the
+    NaN) of the formula, everything else is finite."""
+    leaves, dy = inputs(rows, c, f, dtype, dtype, c)
+    dy[rows // 2, f // 3] = float("inf")
+    got = torch.autograd.grad(ff.gated_feed_forward(*leaves), leaves, dy)
+    for name, a, b in zip(("dx", "dwg", "dwu", "dbg", "dbu"), got, exact(leaves, dy)[1:]):
+        a = a.double()
+        same = torch.where(torch.isfinite(b), torch.isfinite(a), (a == b) | (torch.isnan(a) & torch.isnan(b)))
+        assert bool(same.all()), (name, int((~same).sum()))
