@@ -799,8 +799,9 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
  * stride x_ld), dw_* [c, f], db_* [f] (parameter type) are not NULL; dy has row stride y_ld.  For bfloat16 the gradients of the
  * projections enter the products of dx and dw as two bfloat16 terms each (off by at most 2^-16); bias gradients are sums of the
  * unrounded ones.
- * Results are the same on every call (no atomics).  x, w_gate, w_up and ws 16-byte aligned; at most 65536 channels and units and
- * 2^31 - 1 rows, tensors may pass 2 GiB.  ws: ssmi_gated_ff_workspace_bytes(d, backward) (0 = none; 0 for a refused descriptor too).
+ * Results are the same on every call (no atomics).  x, w_gate, w_up and ws 16-byte aligned; at most 65536 channels and units,
+ * 2^31 - 1 rows and (c + 128) ceil8(f) 4 < 2^31 (a kernel's bytes in float32), other tensors may pass 2 GiB.
+ * ws: ssmi_gated_ff_workspace_bytes(d, backward) (0 = none; 0 for a refused descriptor too).
  * A few rows are answered by a kernel that only streams the parameters.  No counterpart in the reference. */
 enum { SSMI_GATE_SWISH = 0, SSMI_GATE_GELU = 1, SSMI_GATE_RELU = 2, SSMI_GATE_SIGMOID = 3 };
 typedef struct ssmi_gated_desc {

@@ -585,6 +585,13 @@ __global__ __launch_bounds__(64 * WAVES) void gate_rows_kernel(GateArgs a) {
 static inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// The tile loop asks for kStages K steps past the last one, at most 128 memory rows of an operand whose K runs over rows.  Their lanes are
+// switched off by an offset past the descriptor's end, which holds as long as the step's own offset does not pass that end.
+static constexpr int64_t kPastRows = 128, kReach = 0x7FFFFFFF;
+template <typename S> constexpr int64_t past_rows(int es) { return (int64_t)S::kStages * S::kStep / es; }
+static_assert(past_rows<GateShape<2, 1>>(2) <= kPastRows && past_rows<GateShape<2, 2>>(2) <= kPastRows && past_rows<GateShape<2, 4>>(2) <= kPastRows &&
+              past_rows<ProductShape<2, 1>>(2) <= kPastRows && past_rows<ProductShape<2, 2>>(2) <= kPastRows && past_rows<ProductShape<2, 4>>(2) <= kPastRows, "");
+
 // Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
 //   gate: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
 //   no tile of 128 rows or channels where there are 64 (131k x 64 -> 256 float32, dx 142 -> 103 us, dW 127 -> 90)
@@ -664,9 +671,9 @@ static GatePlan gate_plan(const ssmi_gated_desc* d) {
   int64_t strips = ceil_div64(512, ceil_div64(2 * p.fp, 128) * ceil_div64(d->c, q_side(p.dw_tile)));
   strips = strips < most ? strips : most;
   strips = strips > least ? strips : least;
-  // a strip is addressed with 32-bit offsets from its first row: under 2^31 - 2^27 bytes of [dg | du] and of x
+  // a strip is addressed with 32-bit offsets from its first row, and the loop asks for kPastRows more of [dg | du] and of x
   const int64_t row_bytes = p.es * std::max<int64_t>(sides * (int64_t)p.fp, p.pad_x ? p.cp : d->x_ld);
-  const int64_t reach = std::max<int64_t>(((1ll << 31) - (1ll << 27)) / row_bytes / 64 * 64, 64);
+  const int64_t reach = std::max<int64_t>((kReach / row_bytes - kPastRows) / 64 * 64, 64);
   p.strip_rows = std::min(up_to(ceil_div64(d->rows, strips), 64), reach);
   p.strips = (int)ceil_div64(d->rows, p.strip_rows);
   p.part_bytes = up256((size_t)p.strips * d->c * 2 * p.fp * 4);
@@ -690,7 +697,7 @@ static ssmi_status check_desc(const char* who, const ssmi_gated_desc* d) {
   SSMI_REQUIRE(d->dtype == SSMI_F32 || d->dtype == SSMI_BF16, SSMI_E_UNSUPPORTED, "%s: unknown activation dtype %d", who, d->dtype);
   SSMI_REQUIRE(d->param_dtype == SSMI_F32 || (d->param_dtype == SSMI_BF16 && d->dtype == SSMI_BF16), SSMI_E_UNSUPPORTED,
                "%s: parameters are float32, or bfloat16 under bfloat16 activations", who);
-  SSMI_REQUIRE((int64_t)d->c * up_to(d->f, 8) * 4 < (1ll << 31), SSMI_E_UNSUPPORTED, "%s: a kernel of 2 GiB or more", who);
+  SSMI_REQUIRE((d->c + kPastRows) * up_to(d->f, 8) * 4 <= kReach, SSMI_E_UNSUPPORTED, "%s: a kernel that comes within %lld rows of 2 GiB", who, (long long)kPastRows);
   return SSMI_OK;
 }
 

@@ -1,0 +1,40 @@
+"""Limits of the row operators that keep every address in reach, checked without a GPU: by what is refused and by the workspaces asked for."""
+import ctypes as C
+import importlib
+
+import pytest
+
+_lib = importlib.import_module("semantic-segmentation_amd._lib")
+P = 0x1000      # a pointer that no refused call follows
+
+
+def desc(**kw):
+    v = dict(rows=1000, x_ld=kw["c"], y_ld=kw["f"], act=0, dtype=0, param_dtype=0)
+    v.update(kw)
+    return _lib.GatedDesc(*(v[n] for n, _ in _lib.GatedDesc._fields_))
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_kernels_leave_room_for_the_steps_past_their_end(dtype):
+    """The tile loop's last requests lie up to 128 rows behind the kernel; their offsets have to stay in 31 bits."""
+    L = _lib.lib()
+    f = 65528
+    last = (2 ** 31 - 1) // (4 * f) - 128
+    assert L.gated_ff_workspace_bytes(C.byref(desc(c=last, f=f, dtype=dtype)), 1) > 0
+    for c in (last + 1, 8192):
+        d = desc(c=c, f=f, dtype=dtype)
+        assert c * f * 4 < 2 ** 31 and L.gated_ff_workspace_bytes(C.byref(d), 1) == 0
+        with pytest.raises(_lib.SsmiError, match="2 GiB"):
+            L.gated_ff_fwd(C.byref(d), P, P, P, None, None, P, P, 1 << 50, None)
+
+
+@pytest.mark.parametrize("dtype,es", [(0, 4), (1, 2)])
+def test_strips_of_the_weight_gradient_leave_room_for_the_steps_past_their_end(dtype, es):
+    """Rows 2^20 values apart: a strip and 128 rows more stay in 31 bits.  The number of strips shows in the workspace, 4 * c * 2 fp bytes each."""
+    L = _lib.lib()
+    rows, c, f = 1000000, 16, 16
+    wide, dense = (L.gated_ff_workspace_bytes(C.byref(desc(rows=rows, x_ld=ld, c=c, f=f, dtype=dtype)), 1) for ld in (1 << 20, c))
+    usual = -(-rows // 1984)      # 512 strips of whole 64 rows
+    strips = usual + (wide - dense) // (4 * c * 2 * f)
+    longest = (2 ** 31 - 1) // (es << 20) - 128
+    assert strips * longest >= rows, (strips, longest)
