@@ -32,8 +32,10 @@ struct ProductShape {
 template <int SP, int SQ>
 struct GateShape {
   static constexpr int kStep = SQ == 1 ? 128 : 64, kStages = SQ == 4 ? 3 : 2, kAtOnce = SQ == 4 ? 2 : 1, kPerCu = SQ == 4 ? 2 : 3;
-  static constexpr bool kChunks = false;      // K = channels: a running sum is as exact as the plain form's
 };
+// float32 sums over more than kChunk channels go in chunks, whose registers leave two of the larger tiles to a CU (16k x 512 -> 1024 forward
+// 259 -> 267 us, 8k x 1024 -> 1024 247 -> 258); shorter ones have one chunk and stay with three
+template <typename T, int SP, int SQ, bool LONG> constexpr int gate_per_cu() { return LONG && sizeof(T) == 4 && SQ == 2 ? 2 : GateShape<SP, SQ>::kPerCu; }
 
 struct GateArgs {
   const void *x, *wg, *wu;      // x [rows][x_ld], W [c][w_ld], activation type
@@ -59,9 +61,10 @@ __device__ __forceinline__ float rest_of(float v) {
   return __builtin_fabsf(first) < INFINITY ? v - first : 0.f;
 }
 
-template <typename T, int SP, int SQ>
+template <typename T, int SP, int SQ, bool LONG>
 struct GateSides : GateShape<SP, SQ> {
   using GateShape<SP, SQ>::kStep;
+  static constexpr bool kChunks = LONG;
   static constexpr int kHalf = SP * 32;      // units of a tile
   typedef Operand<T, kHalf, true, kStep> W;
   typedef Operand<T, SQ * 64, false, kStep> X;
@@ -83,10 +86,10 @@ struct GateSides : GateShape<SP, SQ> {
   __device__ __forceinline__ u32x4 q(lds_bytes s, int j, int ks) const { return rx.get(s + 2 * W::kBytes, wq * SQ + j, ks); }
 };
 
-template <typename T, int SP, int SQ, bool BWD>
-__global__ __launch_bounds__(256, (GateShape<SP, SQ>::kPerCu)) void gate_kernel(GateArgs a) {
+template <typename T, int SP, int SQ, bool BWD, bool LONG>
+__global__ __launch_bounds__(256, (gate_per_cu<T, SP, SQ, LONG>())) void gate_kernel(GateArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  typedef GateSides<T, SP, SQ> S;
+  typedef GateSides<T, SP, SQ, LONG> S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const TileAt at = tile_at(spread_blocks(blockIdx.x, gridDim.x), a.np, a.nq);
   const int64_t m0 = (int64_t)at.q * (SQ * 64);
@@ -747,15 +750,22 @@ static constexpr int tile_lds() {
   return stages > rows ? stages : rows;
 }
 
-template <typename T, int SP, int SQ, bool BWD>
-static ssmi_status launch_gate_as(GateArgs a, hipStream_t st) {
-  typedef GateSides<T, SP, SQ> S;
+template <typename T, int SP, int SQ, bool BWD, bool LONG>
+static ssmi_status launch_gate_long(GateArgs a, hipStream_t st) {
+  typedef GateSides<T, SP, SQ, LONG> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
   SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d units are too many for one launch", (long long)a.rows, a.f);
-  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
+  hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD, LONG>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
+}
+template <typename T, int SP, int SQ, bool BWD>
+static ssmi_status launch_gate_as(const GateArgs& a, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) {
+    if (a.c > kChunk) return launch_gate_long<T, SP, SQ, BWD, true>(a, st);
+  }
+  return launch_gate_long<T, SP, SQ, BWD, false>(a, st);
 }
 template <typename T, bool BWD>
 static ssmi_status launch_gate(Tile t, const GateArgs& a, hipStream_t st) {
