@@ -756,6 +756,7 @@ static ssmi_status launch_gate_long(GateArgs a, hipStream_t st) {
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
   SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d units are too many for one launch", (long long)a.rows, a.f);
+  set_last_kernel("gate_kernel<%s, %d, %d, %s>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ, BWD ? "backward" : "forward");
   hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD, LONG>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
@@ -780,6 +781,7 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
   SSMI_REQUIRE((int64_t)a.np * a.nq * a.strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
+  set_last_kernel("gate_dx_kernel<%s, %d, %d>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ);
   hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)a.strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
@@ -790,6 +792,7 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
   SSMI_REQUIRE((int64_t)a.np * a.nq * strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
+  set_last_kernel("gate_dw_kernel<%s, %d, %d>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ);
   hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;

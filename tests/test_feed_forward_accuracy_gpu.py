@@ -1,5 +1,6 @@
 """How exact the gated feed-forward unit's results are, by norms of whole tensors against float64 (computed on the GPU).  The bounds come
 from the arithmetic and stand at each test."""
+import ctypes as C
 import importlib
 
 import pytest
@@ -83,3 +84,47 @@ def test_float32_sums_over_many_channels(rows, c, f):
     assert off(y, want[0]) <= 8e-7, off(y, want[0])
     for name, a, b, w in zip(("y", "dx", "dwg", "dwu", "dbg", "dbu"), got, other, want):
         assert off(a, w) <= off(b, w) or c < 1024, (name, off(a, w), off(b, w))
+
+
+def kernels_taken(leaves, dy):
+    """Names of the kernels that a forward call, a backward call for nothing, for dx alone and for the kernels' gradients alone launch last."""
+    _lib = importlib.import_module("semantic-segmentation_amd._lib")
+    L = _lib.lib()
+    x, wg, wu, bg, bu = (t.detach() for t in leaves)
+    (rows, c), f, code = x.shape, wg.shape[1], 1 if x.dtype == torch.bfloat16 else 0
+    d = C.byref(_lib.GatedDesc(rows, c, f, c, f, 0, code, code))
+    n = max(L.gated_ff_workspace_bytes(d, k) for k in (0, 1))
+    ws, y, dx, dw = torch.empty(n, dtype=torch.uint8, device=DEV), torch.empty_like(dy), torch.empty_like(x), torch.empty_like(wg)
+    st = torch.cuda.current_stream().cuda_stream
+    front = [d, *(t.data_ptr() for t in (x, wg, wu, bg, bu))]
+    names = []
+    L.gated_ff_fwd(*front, y.data_ptr(), ws.data_ptr(), n, st)
+    names.append(L.last_kernel().decode())
+    for a, b in ((None, None), (dx.data_ptr(), None), (None, dw.data_ptr())):
+        L.gated_ff_bwd(*front, dy.data_ptr(), a, b, None, None, None, ws.data_ptr(), n, st)
+        names.append(L.last_kernel().decode())
+    torch.cuda.synchronize()
+    return names
+
+
+@pytest.mark.parametrize("dtype,rows,c,f,tiles", [
+    (torch.bfloat16, 50000, 144, 2800, ("2, 4", "2, 4", "4, 4", "2, 4")),      # the largest tiles, every axis with a remainder
+    (torch.bfloat16, 49152, 256, 2816, ("2, 4", "2, 4", "4, 4", "2, 4")),      # the same, whole tiles
+    (torch.bfloat16, 4099, 1000, 1500, ("2, 4", "2, 4", "2, 2", "2, 2")),
+    (torch.bfloat16, 33000, 64, 192, ("2, 4", "2, 4", "1, 1", "2, 1")),
+    (torch.bfloat16, 300, 100, 270, ("2, 1", "2, 1", "1, 1", "2, 1")),
+    *((dt, 8200, 264, 520, ("2, 2", "2, 2", "2, 1", "2, 2")) for dt in (torch.bfloat16, torch.float32)),
+    (torch.float32, 40000, 144, 600, ("2, 2", "2, 2", "2, 2", "2, 2")),
+    (torch.float32, 33000, 64, 192, ("2, 2", "2, 2", "1, 1", "2, 1")),
+    (torch.float32, 300, 100, 270, ("2, 1", "2, 1", "1, 1", "2, 1"))])
+def test_every_tile_of_the_gradients(dtype, rows, c, f, tiles):
+    """The bounds are those of the tests above; float32 gradients sum at most 4096 rows or 2 f units in chunks: under 1e-6."""
+    leaves, dy = inputs(rows, c, f, dtype, dtype, c)
+    t = "bf16" if dtype == torch.bfloat16 else "float"
+    assert kernels_taken(leaves, dy) == ["gate_kernel<{}, {}, forward>".format(t, tiles[0]), "gate_kernel<{}, {}, backward>".format(t, tiles[1]),
+                                         "gate_dx_kernel<{}, {}>".format(t, tiles[2]), "gate_dw_kernel<{}, {}>".format(t, tiles[3])]
+    y = ff.gated_feed_forward(*leaves)
+    for name, a, b in zip(("y", "dx", "dwg", "dwu", "dbg", "dbu"), (y, *torch.autograd.grad(y, leaves, dy)), exact(leaves, dy)):
+        r = off(a, b) if dtype == torch.float32 else off(a, b.to(dtype).double())
+        assert r <= (1e-6 if dtype == torch.float32 else 2.0 ** -11), (name, r)
+        assert bool(torch.isfinite(a).all())
