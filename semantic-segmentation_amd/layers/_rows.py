@@ -5,6 +5,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import BF16, F32
 
@@ -24,6 +25,15 @@ def require_gpu(t, who: str) -> None:
         raise TypeError("{}: a torch tensor expected, got {}".format(who, type(t).__name__))
     if not t.is_cuda:      # the error of the pooling layers
         raise NotImplementedError("{} works only on GPU".format(who))
+
+
+def refuse_tangents(who: str, *tensors) -> None:
+    """The kernels have no forward-mode derivative: a tensor with a tangent would lose it without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # outside every level no tensor has one
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("{}: an input carries a tangent, and there is no forward-mode derivative".format(who))
 
 
 def on(t: torch.Tensor):

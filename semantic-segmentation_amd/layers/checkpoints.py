@@ -15,7 +15,7 @@ import ctypes as C
 import torch
 
 from .._lib import BnParams, lib
-from ._rows import dtype_code, on, require_gpu, rows_of, stream_of, vector
+from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of, vector
 
 GROUP = 32
 _ACTS = {"none": 0, "prelu": 1, "leaky": 2}
@@ -79,8 +79,10 @@ class Checkpoint8(object):
 
 
 def store_8bit(x: torch.Tensor) -> Checkpoint8:
-    """The tensor's checkpoint.  `x`: float32 or bfloat16 with the channels on its last axis, dense or a channel slice of a wider tensor."""
+    """The tensor's checkpoint.  `x`: float32 or bfloat16 with the channels on its last axis, dense or a channel slice of a wider tensor.
+    What is restored from it is detached: a checkpoint serves a backward pass and is no part of a graph."""
     require_gpu(x, "store_8bit")
+    refuse_tangents("store_8bit", x)
     code = dtype_code(x, "store_8bit")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("store_8bit: a tensor with channels on its last axis expected, got shape {}".format(tuple(x.shape)))

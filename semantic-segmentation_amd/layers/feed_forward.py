@@ -15,7 +15,7 @@ import functools
 import torch
 
 from .._lib import BF16, GatedDesc, lib
-from ._rows import dtype_code, on, require_gpu, rows_of, stream_of
+from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of
 from .checkpoints import store_8bit
 from .microscaled import MX4Weights, mx4_gated
 
@@ -110,6 +110,7 @@ def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="swis
     backward pass.  w_gate and w_up may be MX4Weights (biases then float32): answering on 4-bit products."""
     who = "gated_feed_forward"
     require_gpu(x, who)
+    refuse_tangents(who, x, w_gate, w_up, b_gate, b_up)
     if activation not in ACTIVATIONS:
         raise ValueError("{}: activation must be one of {}, got {!r}".format(who, sorted(ACTIVATIONS), activation))
     if checkpoint not in (None, "8bit"):

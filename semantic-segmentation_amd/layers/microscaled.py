@@ -13,7 +13,7 @@ import functools
 import torch
 
 from .._lib import lib
-from ._rows import dtype_code, on, require_gpu, rows_of, stream_of, vector
+from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of, vector
 
 BLOCK = 32
 _GATES = {"swish": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -53,6 +53,7 @@ class MX4Weights(object):
 def quantize_mx4_weights(w: torch.Tensor) -> MX4Weights:
     who = "quantize_mx4_weights"
     require_gpu(w, who)
+    refuse_tangents(who, w)
     code = dtype_code(w, who)
     if w.dim() != 2 or 0 in w.shape:
         raise ValueError("{}: a kernel [k, n] expected, got shape {}".format(who, tuple(w.shape)))
@@ -68,6 +69,7 @@ def quantize_mx4_weights(w: torch.Tensor) -> MX4Weights:
 
 def _operand(x, w: MX4Weights, who, *biases):
     require_gpu(x, who)
+    refuse_tangents(who, x, *biases)
     if not isinstance(w, MX4Weights):
         raise TypeError("{}: MX4Weights expected, got {}".format(who, type(w).__name__))
     if x.dim() < 1 or x.shape[-1] != w.k or w.codes.device != x.device:
