@@ -16,7 +16,7 @@ import torch
 
 from .._lib import BF16, GatedDesc, lib
 from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of
-from .checkpoints import store_8bit
+from .checkpoints import Checkpoint8, store_8bit
 from .microscaled import MX4Weights, mx4_gated
 
 ACTIVATIONS = {"swish": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -70,17 +70,18 @@ class _GatedFn(torch.autograd.Function):
             bg, bu = bg.contiguous(), bu.contiguous()
         y = _forward(x, wg, wu, bg, bu, act)
         ctx.act = act
-        ctx.kept = None if checkpoint is None else store_8bit(x)
-        ctx.save_for_backward(x if checkpoint is None else None, wg, wu, bg, bu)
+        # the checkpoint's tensors are saved as any others: gone behind the backward pass, seen by saved-tensor hooks
+        kept = None if checkpoint is None else store_8bit(x)
+        ctx.kept_as = None if kept is None else (kept.shape, kept.dtype)
+        ctx.save_for_backward(wg, wu, bg, bu, *((x,) if kept is None else (kept.codes, kept.scales)))
         return y
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():      # create_graph=True: what follows is not recorded
             raise RuntimeError("gated_feed_forward has no second derivative")
-        x, wg, wu, bg, bu = ctx.saved_tensors
-        if x is None:
-            x = ctx.kept.restore()
+        wg, wu, bg, bu, *kept = ctx.saved_tensors
+        x = kept[0] if ctx.kept_as is None else Checkpoint8(*kept, *ctx.kept_as).restore()
         nx, ng, nu, nbg, nbu = ctx.needs_input_grad[:5]
         c, f = wg.shape
         t, rows, ld = _aligned_rows(x)

@@ -41,3 +41,27 @@ def test_tangents_are_refused(grad):
         assert torch.equal(ff.gated_feed_forward(*free), want)
         ms.mx4_dense(free[0], q[0]), cp.store_8bit(free[0])
     assert torch.equal(ff.gated_feed_forward(*free), want)
+
+
+def test_a_checkpoint_lives_as_long_as_the_backward_pass_needs_it():
+    """Its tensors are saved tensors: hooks see them, they are gone behind a backward pass (while the output lives), and a second pass without
+    retain_graph is refused as it is without a checkpoint."""
+    rows, c = 4096, 512      # 2 MiB of codes, a block of its own
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(rows, c, generator=g).to(DEV).requires_grad_()
+    w = [torch.randn(c, 8, generator=g).to(DEV).requires_grad_() for _ in range(2)]
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append((t.dtype, tuple(t.shape))) or t, lambda t: t):
+        y = ff.gated_feed_forward(x, *w, checkpoint="8bit")
+    assert (torch.uint8, (rows, c)) in seen and (torch.uint8, (rows, c // 32)) in seen and (torch.float32, (rows, c)) not in seen
+    for checkpoint in (None, "8bit"):
+        y = ff.gated_feed_forward(x, *w, checkpoint=checkpoint)
+        first = torch.autograd.grad(y.sum(), [x, *w], retain_graph=True)
+        before = torch.cuda.memory_allocated()
+        second = torch.autograd.grad(y.sum(), [x, *w])
+        assert all(torch.equal(a, b) for a, b in zip(first, second))
+        del second
+        freed = before - torch.cuda.memory_allocated()
+        assert freed >= (rows * c if checkpoint else 0), freed
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y.sum(), [x, *w])
