@@ -51,9 +51,12 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def rows_of(t: torch.Tensor):
-    """(tensor, rows, row stride): `t` itself where its leading axes step evenly over rows of contiguous channels - a channel
-    slice of a wider tensor, for instance -, a contiguous copy otherwise."""
+FAR = 1 << 20      # the products address a tile's rows with 32-bit offsets: values from one row to the next
+
+
+def rows_of(t: torch.Tensor, most: int = 1 << 62):
+    """(tensor, rows, row stride): `t` itself where its leading axes step evenly, by at most `most` values, over rows of contiguous
+    channels - a channel slice of a wider tensor, for instance -, a contiguous copy otherwise."""
     c = t.shape[-1]
     if t.is_contiguous():
         return t, t.numel() // c if c else 0, c
@@ -69,7 +72,7 @@ def rows_of(t: torch.Tensor):
                 break
             step *= size
         else:
-            if ld is not None and ld >= c:
+            if ld is not None and c <= ld <= most:
                 return t, t.numel() // c, ld
     t = t.contiguous()
     return t, t.numel() // c if c else 0, c

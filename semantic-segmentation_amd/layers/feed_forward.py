@@ -15,7 +15,7 @@ import functools
 import torch
 
 from .._lib import BF16, GatedDesc, lib
-from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of
+from ._rows import FAR, dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of
 from .checkpoints import Checkpoint8, store_8bit
 from .microscaled import MX4Weights, mx4_gated
 
@@ -28,7 +28,7 @@ def _ptr(t):
 
 def _aligned_rows(x):
     """rows_of with the 16-byte alignment that the products ask of their operands."""
-    t, rows, ld = rows_of(x)
+    t, rows, ld = rows_of(x, FAR)
     if t.data_ptr() % 16:
         t = t.contiguous() if not t.is_contiguous() else t.clone()
         ld = t.shape[-1]
@@ -89,7 +89,7 @@ class _GatedFn(torch.autograd.Function):
             return (torch.zeros_like(x) if nx else None, *(torch.zeros_like(p) if n else None for p, n in ((wg, ng), (wu, nu), (bg, nbg), (bu, nbu))), None, None)
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
-        dt, _, dy_ld = rows_of(dy)
+        dt, _, dy_ld = rows_of(dy, FAR)
         if nx and ld != c:      # the row stride of dx is that of x
             t, ld = _dense(t), c
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if nx else None

@@ -13,7 +13,7 @@ import functools
 import torch
 
 from .._lib import lib
-from ._rows import dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of, vector
+from ._rows import FAR, dtype_code, on, refuse_tangents, require_gpu, rows_of, stream_of, vector
 
 BLOCK = 32
 _GATES = {"swish": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -76,7 +76,7 @@ def _operand(x, w: MX4Weights, who, *biases):
         raise ValueError("{}: x [..., {}] on {} expected, got {} on {}".format(who, w.k, w.codes.device, tuple(x.shape), x.device))
     if torch.is_grad_enabled() and (x.requires_grad or any(isinstance(b, torch.Tensor) and b.requires_grad for b in biases)):
         raise ValueError("{}: 4-bit products have no backward pass; call them under torch.no_grad() or on detached tensors".format(who))
-    t, rows, ld = rows_of(x)
+    t, rows, ld = rows_of(x, FAR)
     return t, rows, ld, torch.empty(x.shape[:-1] + (w.n,), dtype=x.dtype, device=x.device)
 
 

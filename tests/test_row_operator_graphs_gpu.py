@@ -65,3 +65,24 @@ def test_a_checkpoint_lives_as_long_as_the_backward_pass_needs_it():
         assert freed >= (rows * c if checkpoint else 0), freed
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(y.sum(), [x, *w])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_more_than_2_20_values_apart(dtype):
+    """The first pixel of every image of a batch: rows a whole image apart.  Results are those of a dense copy."""
+    x, wg, wu, bg, bu = (t.to(dtype) for t in tensors(rows=20, c=64))
+    images = torch.zeros(20, 130 * 130, 64, dtype=dtype, device=DEV)
+    images[:, 0] = x
+    leaf = images.requires_grad_()
+    view = leaf[:, 0]
+    assert view.stride(0) > 1 << 20
+    y, want = ff.gated_feed_forward(view, wg, wu, bg, bu), ff.gated_feed_forward(x, wg, wu, bg, bu)
+    assert torch.equal(y, want)
+    dy = torch.ones(20, 130 * 2000, 24, dtype=dtype, device=DEV)[:, 0]      # and a gradient with rows as far apart
+    (d,) = torch.autograd.grad(y, leaf, dy)
+    x.requires_grad_()
+    (want,) = torch.autograd.grad(ff.gated_feed_forward(x, wg, wu, bg, bu), x, torch.ones_like(y))
+    assert torch.equal(d[:, 0], want) and not bool(d[:, 1:].any())
+    q = ms.quantize_mx4_weights(wg)
+    assert torch.equal(ms.mx4_dense(view.detach(), q), ms.mx4_dense(x.detach(), q))
+    assert torch.equal(cp.store_8bit(view).restore(), cp.store_8bit(x).restore())

@@ -51,3 +51,16 @@ def test_tangents_are_found_on_any_device():
         with pytest.raises(ValueError, match="call: an input carries a tangent"):
             rows.refuse_tangents("call", None, forward_ad.make_dual(x, x))
     rows.refuse_tangents("call", x)
+
+
+def test_rows_far_apart_are_copied_where_the_products_cannot_reach_them():
+    rows = importlib.import_module("semantic-segmentation_amd.layers._rows")
+    far = torch.empty(1).expand(1).as_strided((3, 8), (0, 0))      # only shapes and strides count
+    near, over = (torch.empty(2 * s + 8, dtype=torch.uint8).as_strided((3, 8), (s, 1)) for s in (1 << 20, (1 << 20) + 1))
+    t, n, ld = rows.rows_of(near, rows.FAR)
+    assert t is near and (n, ld) == (3, 1 << 20)
+    t, n, ld = rows.rows_of(over, rows.FAR)
+    assert t is not over and (n, ld) == (3, 8) and torch.equal(t, over)
+    t, n, ld = rows.rows_of(over)      # the checkpoints reach every row
+    assert t is over and ld == (1 << 20) + 1
+    assert rows.rows_of(far)[2] == 8
