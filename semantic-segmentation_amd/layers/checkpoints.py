@@ -28,7 +28,22 @@ class Checkpoint8(object):
     __slots__ = ("codes", "scales", "shape", "dtype")
 
     def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, torch.Size(shape), dtype
+        shape = torch.Size(shape)
+        c = shape[-1] if len(shape) else 0
+        rows = shape.numel() // c if c else 0
+        want = (rows, c), (rows, (c + GROUP - 1) // GROUP)
+        if c < 1 or dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != torch.uint8 or tuple(t.shape) != s for t, s in zip((codes, scales), want)) or \
+                codes.device != scales.device:
+            raise ValueError("Checkpoint8: codes uint8 {} and scales uint8 {} on one device expected for a {} tensor of shape {}, got {} {} and {} {}".format(
+                *want, dtype, tuple(shape), codes.dtype, tuple(codes.shape), scales.dtype, tuple(scales.shape)))
+        self.codes, self.scales, self.shape, self.dtype = codes.contiguous(), scales.contiguous(), shape, dtype
+
+    @classmethod
+    def _made(cls, codes, scales, shape, dtype):
+        """Of tensors that store_8bit made."""
+        self = object.__new__(cls)
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+        return self
 
     @property
     def nbytes(self) -> int:
@@ -43,6 +58,7 @@ class Checkpoint8(object):
 
     def restore(self, out=None) -> torch.Tensor:
         y = self._target(out, "restore")
+        require_gpu(y, "restore")
         if y.numel():
             rows, c = self.codes.shape
             with on(y):
@@ -65,8 +81,11 @@ class Checkpoint8(object):
             if len(self.shape) < 2:
                 raise ValueError("{}: a dropout table needs an axis of images".format(who))
             drop = vector(drop, self.shape[0] * c, self.codes, who, "drop")
+            if tuple(drop.shape) != (self.shape[0], c):
+                raise ValueError("{}: drop must be [{}, {}], got {}".format(who, self.shape[0], c, tuple(drop.shape)))
             for d in self.shape[1:-1]:
                 hw *= d
+        require_gpu(self.codes, who)
         y, out = self._target(None, who), self._target(None, who)
         if y.numel():
             rows = self.codes.shape[0]
@@ -93,4 +112,4 @@ def store_8bit(x: torch.Tensor) -> Checkpoint8:
     if rows:
         with on(x):
             lib().act8_store(t.data_ptr(), ld, rows, c, code, codes.data_ptr(), scales.data_ptr(), stream_of(x))
-    return Checkpoint8(codes, scales, x.shape, x.dtype)
+    return Checkpoint8._made(codes, scales, x.shape, x.dtype)

@@ -64,3 +64,24 @@ def test_rows_far_apart_are_copied_where_the_products_cannot_reach_them():
     t, n, ld = rows.rows_of(over)      # the checkpoints reach every row
     assert t is over and ld == (1 << 20) + 1
     assert rows.rows_of(far)[2] == 8
+
+
+def test_checkpoints_made_by_hand_have_to_fit_together():
+    """What restore() reads goes by the shape: codes and scales that are shorter would be read past their ends."""
+    cp = importlib.import_module("semantic-segmentation_amd.layers.checkpoints")
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8)      # noqa: E731
+    kept = cp.Checkpoint8(u8(40, 6).t(), u8(6, 2), (2, 3, 40), torch.bfloat16)
+    assert kept.codes.is_contiguous() and kept.shape == (2, 3, 40)
+    for codes, scales, shape, dtype in ((u8(5, 40), u8(6, 2), (2, 3, 40), torch.float32), (u8(6, 40), u8(6, 1), (2, 3, 40), torch.float32),
+                                        (u8(6, 40), u8(6, 2), (3, 3, 40), torch.float32), (u8(6, 40), u8(6, 2), (6, 41), torch.float32),
+                                        (u8(6, 40), u8(6, 2), (6, 40), torch.float16), (u8(6, 40).float(), u8(6, 2), (6, 40), torch.float32),
+                                        (u8(6, 40), u8(6, 2), (), torch.float32), (u8(240), u8(6, 2), (6, 40), torch.float32),
+                                        (u8(6, 40), u8(6, 2).to("meta"), (6, 40), torch.float32)):
+        with pytest.raises(ValueError, match="Checkpoint8"):
+            cp.Checkpoint8(codes, scales, shape, dtype)
+    v = torch.ones(40)
+    for call in (kept.restore, lambda: kept.restore_bn_act(v, v, v, v)):
+        with pytest.raises(NotImplementedError):
+            call()
+    with pytest.raises(ValueError, match="drop must be"):      # a table of the other order has as many values
+        kept.restore_bn_act(v, v, v, v, drop=torch.ones(40, 2))
