@@ -54,9 +54,14 @@ class Checkpoint8(object):
             return torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
         if out.shape != self.shape or out.dtype != self.dtype or out.device != self.codes.device or not out.is_contiguous():
             raise ValueError("{}: out must be a dense {} tensor of shape {} on {}".format(who, self.dtype, tuple(self.shape), self.codes.device))
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("{}: out must not ask for gradients".format(who))
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)      # what a graph saved of it is stale from here on
         return out
 
     def restore(self, out=None) -> torch.Tensor:
+        """The tensor back, in `out` (dense, of its shape and type) where that is given."""
         y = self._target(out, "restore")
         require_gpu(y, "restore")
         if y.numel():

@@ -86,3 +86,19 @@ def test_rows_more_than_2_20_values_apart(dtype):
     q = ms.quantize_mx4_weights(wg)
     assert torch.equal(ms.mx4_dense(view.detach(), q), ms.mx4_dense(x.detach(), q))
     assert torch.equal(cp.store_8bit(view).restore(), cp.store_8bit(x).restore())
+
+
+def test_restore_into_a_tensor_counts_as_a_change_of_it():
+    """A graph that saved the target must not go on with what it finds there, and a leaf that learns is no target."""
+    x, w = torch.randn(6, 40, device=DEV), torch.randn(6, 40, device=DEV, requires_grad=True)
+    kept, buf = cp.store_8bit(x), torch.zeros(6, 40, device=DEV)
+    y = (buf * w).sum()
+    assert kept.restore(out=buf) is buf and torch.equal(buf, kept.restore())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="gradients"):
+        kept.restore(out=w)
+    with torch.no_grad():
+        assert torch.equal(kept.restore(out=w), buf)
+    with torch.inference_mode():
+        assert torch.equal(kept.restore(out=torch.zeros(6, 40, device=DEV)), buf)
