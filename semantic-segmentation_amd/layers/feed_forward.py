@@ -161,12 +161,14 @@ class GatedFeedForward2D(object):
     def build(self, input_shape, device="cuda"):
         c = input_shape[-1]
         g = torch.Generator().manual_seed(self.seed)
-        self.weights = [(torch.randn(c, self.units, generator=g) * (2.0 / c) ** 0.5).to(device).requires_grad_() for _ in range(2)]
-        if self.use_bias:
-            self.weights += [torch.zeros(self.units, device=device, requires_grad=True) for _ in range(2)]
+        with torch.inference_mode(False):      # weights made in a first call that only answers can learn later
+            self.weights = [(torch.randn(c, self.units, generator=g) * (2.0 / c) ** 0.5).to(device).requires_grad_() for _ in range(2)]
+            if self.use_bias:
+                self.weights += [torch.zeros(self.units, device=device, requires_grad=True) for _ in range(2)]
 
     def set_weights(self, weights, device="cuda"):
-        ws = [torch.as_tensor(w, dtype=torch.float32).detach().clone().to(device) for w in weights]
+        with torch.inference_mode(False):
+            ws = [torch.as_tensor(w, dtype=torch.float32).detach().clone().to(device) for w in weights]
         if len(ws) != (4 if self.use_bias else 2) or any(w.dim() != 2 or w.shape != ws[0].shape or w.shape[1] != self.units for w in ws[:2]) or \
                 any(b.shape != (self.units,) for b in ws[2:]):
             raise ValueError("expected {} with {} units, got shapes {}".format("two kernels and two biases" if self.use_bias else "two kernels", self.units,
