@@ -704,6 +704,16 @@ static ssmi_status check_desc(const char* who, const ssmi_gated_desc* d) {
   return SSMI_OK;
 }
 
+// every launch of a call inside kMostBlocks, checked in front of the first
+static ssmi_status check_launches(const char* who, const ssmi_gated_desc* d, const GatePlan& p, bool dx, bool dw) {
+  int64_t most = ceil_div64(d->rows, q_side(p.gate_tile)) * ceil_div64(d->f, 64);
+  const int64_t dx_side = p.dx_tile == kTile64x64 ? 64 : p.dx_tile == kTile256x256 ? 256 : 128;
+  if (dx) most = std::max(most, ceil_div64(d->rows, q_side(p.dx_tile)) * ceil_div64(d->c, dx_side) * p.dx_strips);
+  if (dw) most = std::max(most, ceil_div64(d->c, q_side(p.dw_tile)) * ceil_div64(2 * p.fp, 128) * p.strips);
+  SSMI_REQUIRE(most < kMostBlocks, SSMI_E_UNSUPPORTED, "%s: %lld rows of %d channels and %d units are too many for one launch", who, (long long)d->rows, d->c, d->f);
+  return SSMI_OK;
+}
+
 static inline bool aligned(const void* p, int b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
 
 // how rows may be stored: 0 value by value, 1 four values at a time, 2 eight
@@ -755,7 +765,6 @@ static ssmi_status launch_gate_long(GateArgs a, hipStream_t st) {
   typedef GateSides<T, SP, SQ, LONG> S;
   a.np = (unsigned)ceil_div64(a.f, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d units are too many for one launch", (long long)a.rows, a.f);
   set_last_kernel("gate_kernel<%s, %d, %d, %s>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ, BWD ? "backward" : "forward");
   hipLaunchKernelGGL((gate_kernel<T, SP, SQ, BWD, LONG>), dim3(a.np * a.nq), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
@@ -780,7 +789,6 @@ static ssmi_status launch_dx_as(GateDxArgs a, hipStream_t st) {
   typedef DxSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(a.c, SP * 64);
   a.nq = (unsigned)ceil_div64(a.rows, SQ * 64);
-  SSMI_REQUIRE((int64_t)a.np * a.nq * a.strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
   set_last_kernel("gate_dx_kernel<%s, %d, %d>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ);
   hipLaunchKernelGGL((gate_dx_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)a.strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
@@ -791,7 +799,6 @@ static ssmi_status launch_dw_as(GateDwArgs a, int strips, hipStream_t st) {
   typedef DwSides<T, SP, SQ> S;
   a.np = (unsigned)ceil_div64(2 * a.fp, SP * 64);
   a.nq = (unsigned)ceil_div64(a.c, SQ * 64);
-  SSMI_REQUIRE((int64_t)a.np * a.nq * strips < kMostBlocks, SSMI_E_UNSUPPORTED, "gated_ff: %lld rows of %d channels are too many for one launch", (long long)a.rows, a.c);
   set_last_kernel("gate_dw_kernel<%s, %d, %d>", sizeof(T) == 2 ? "bf16" : "float", SP, SQ);
   hipLaunchKernelGGL((gate_dw_kernel<T, SP, SQ>), dim3(a.np * a.nq * (unsigned)strips), dim3(256), (tile_lds<S, SP, SQ>()), st, a);
   SSMI_LAUNCH_CHECK();
@@ -940,6 +947,8 @@ ssmi_status ssmi_gated_ff_fwd(const ssmi_gated_desc* d, const void* x, const voi
   SSMI_REQUIRE(aligned(ws, 16), SSMI_E_INVALID_ARG, "gated_ff_fwd: the workspace must be 16-byte aligned");
   SSMI_REQUIRE(takes_rows_kernel(d) || ((aligned(x, 16) || gate_plan(d).pad_x) && ((aligned(w_gate, 16) && aligned(w_up, 16)) || gate_plan(d).pad_w)), SSMI_E_INVALID_ARG,
                "gated_ff_fwd: x and the kernels must be 16-byte aligned");
+  const ssmi_status fits = takes_rows_kernel(d) ? SSMI_OK : check_launches("gated_ff_fwd", d, gate_plan(d), false, false);
+  if (fits != SSMI_OK) return fits;
   return dispatch_dtype(d->dtype, [&](auto tag) -> ssmi_status { return gated_fwd<decltype(tag)>(d, x, w_gate, w_up, b_gate, b_up, y, ws, as_stream(stream)); });
 }
 
@@ -955,6 +964,8 @@ ssmi_status ssmi_gated_ff_bwd(const ssmi_gated_desc* d, const void* x, const voi
   const GatePlan p = gate_plan(d);
   SSMI_REQUIRE((aligned(x, 16) || p.pad_x) && ((aligned(w_gate, 16) && aligned(w_up, 16)) || p.pad_w), SSMI_E_INVALID_ARG,
                "gated_ff_bwd: x and the kernels must be 16-byte aligned");
+  const ssmi_status fits = check_launches("gated_ff_bwd", d, p, dx, dw_gate || dw_up);
+  if (fits != SSMI_OK) return fits;
   return dispatch_dtype(d->dtype, [&](auto tag) -> ssmi_status {
     return gated_bwd<decltype(tag)>(d, x, w_gate, w_up, b_gate, b_up, dy, dx, dw_gate, dw_up, db_gate, db_up, ws, as_stream(stream));
   });

@@ -447,7 +447,6 @@ static ssmi_status launch_tiles(Mx4Args a, hipStream_t st) {
   typedef Mx4Shape<SP, SQ, GATE> S;
   a.np = (unsigned)ceil_div64(a.n, S::kHalf);
   a.nq = (unsigned)ceil_div64(a.rows, S::kQ);
-  SSMI_REQUIRE((int64_t)a.np * a.nq < kMostBlocks, SSMI_E_UNSUPPORTED, "mx4: %lld rows of %d columns are too many for one launch", (long long)a.rows, a.n);
   hipLaunchKernelGGL((mx4_kernel<T, SP, SQ, GATE>), dim3(a.np * a.nq), dim3(256), S::kLds, st, a);
   SSMI_LAUNCH_CHECK();
   return SSMI_OK;
@@ -464,6 +463,8 @@ static ssmi_status mx4_product(const char* who, const void* x, int64_t x_ld, int
   const size_t need = ssmi_mx4_workspace_bytes(rows, k);
   SSMI_REQUIRE(need == 0 || (ws && ws_bytes >= need), SSMI_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
   SSMI_REQUIRE(at16(ws), SSMI_E_INVALID_ARG, "%s: the workspace must be 16-byte aligned", who);
+  SSMI_REQUIRE(ceil_div64(rows, Mx4Shape<2, 2, GATE>::kQ) * ceil_div64(n, Mx4Shape<2, 2, GATE>::kHalf) < kMostBlocks, SSMI_E_UNSUPPORTED,
+               "%s: %lld rows of %d columns are too many for one launch", who, (long long)rows, n);
   a.rows = rows;
   a.n = n;
   a.nb = blocks_of(k);

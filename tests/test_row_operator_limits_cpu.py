@@ -99,3 +99,17 @@ def test_weights_made_under_inference_mode_can_learn():
         assert all(w.requires_grad and w.is_leaf and not w.is_inference() for w in layer.weights)
         (layer.weights[0] * layer.weights[1]).sum().backward()
     assert all(torch.equal(a, b) for a, b in zip(made.weights, again.weights))
+
+
+def test_launches_that_are_too_large_are_refused_in_front_of_the_first():
+    L = _lib.lib()
+    rows = (1 << 30) + 64
+    d = desc(rows=rows, c=8, f=8, dtype=1, param_dtype=1)
+    assert L.gated_ff_workspace_bytes(C.byref(d), 1) > 0
+    with pytest.raises(_lib.SsmiError, match="too many for one launch"):
+        L.gated_ff_bwd(C.byref(d), P, P, P, None, None, P, P, P, P, None, None, P, 1 << 50, None)
+    d = desc(rows=(1 << 31) - 1, c=8, f=8)
+    with pytest.raises(_lib.SsmiError, match="too many for one launch"):
+        L.gated_ff_fwd(C.byref(d), P, P, P, None, None, P, P, 1 << 50, None)
+    with pytest.raises(_lib.SsmiError, match="too many for one launch"):
+        L.mx4_dense(P, 64, (1 << 31) - 1, 64, 8, 0, P, P, None, P, 8, P, 1 << 50, None)
