@@ -1,7 +1,5 @@
-"""float64 restatements of the row operators (8-bit checkpoints, 4-bit microscaled product, gated feed-forward unit): numpy and
-torch on the CPU, test infrastructure only."""
-import math
-
+"""float64 restatement of the row operators' number formats (8-bit checkpoints, 4-bit microscaled product): numpy on the CPU, test
+infrastructure only."""
 import numpy as np
 
 GRID8 = np.array([k * 2.0 ** -9 for k in range(8)] + [(8 + k) * 2.0 ** (e - 3) for e in range(-6, 9) for k in range(8)][:-1])      # e4m3: 0 .. 448
@@ -45,18 +43,3 @@ def quantise(x, kind):
 def codes8(x):
     idx, sign, byte, val = quantise(x, 8)
     return (idx + 128 * sign).astype(np.uint8), byte.astype(np.uint8), val
-
-
-def act(name, v):
-    if name == "swish":
-        return v / (1.0 + np.exp(-v))
-    if name == "gelu":
-        return 0.5 * v * (1.0 + _erf(v / math.sqrt(2.0)))
-    if name == "relu":
-        return np.maximum(v, 0.0)
-    return 1.0 / (1.0 + np.exp(-v))
-
-
-def _erf(v):
-    from scipy.special import erf
-    return erf(v)
