@@ -800,7 +800,7 @@ ssmi_status ssmi_act8_restore_bn_act(const uint8_t* codes, const uint8_t* scales
  * projections enter the products of dx and dw as two bfloat16 terms each (off by at most 2^-16); bias gradients are sums of the
  * unrounded ones.
  * Results are the same on every call (no atomics).  x, w_gate, w_up and ws 16-byte aligned; at most 65536 channels and units,
- * 2^31 - 1 rows and (c + 128) ceil8(f) 4 < 2^31 (a kernel's bytes in float32), other tensors may pass 2 GiB.
+ * 2^31 - 1 rows, row strides of 2^20 and (c + 128) ceil8(f) 4 < 2^31 (a kernel's bytes in float32); other tensors may pass 2 GiB.
  * ws: ssmi_gated_ff_workspace_bytes(d, backward) (0 = none; 0 for a refused descriptor too).
  * A few rows are answered by a kernel that only streams the parameters.  No counterpart in the reference. */
 enum { SSMI_GATE_SWISH = 0, SSMI_GATE_GELU = 1, SSMI_GATE_RELU = 2, SSMI_GATE_SIGMOID = 3 };
@@ -831,7 +831,7 @@ ssmi_status ssmi_gated_ff_bwd(const ssmi_gated_desc* d, const void* x, const voi
  *   ssmi_mx4_dense              y [rows, n] = q(x) w + bias (bias float32 [n] or NULL; y row stride y_ld, type dtype)
  *   ssmi_mx4_gated              y = act(q(x) w_gate + b_gate) * (q(x) w_up + b_up), SSMI_GATE_* activations
  * x is quantised inside the product calls (ws: ssmi_mx4_workspace_bytes(rows, k); 16-byte aligned).  codes 16-byte aligned.  At most
- * 65536 reduction elements and columns and 2^31 - 1 rows; tensors may pass 2 GiB. */
+ * 65536 reduction elements and columns, 2^31 - 1 rows and row strides of 2^20; tensors may pass 2 GiB. */
 ssmi_status ssmi_mx4_quantize(const void* x, int64_t ld, int64_t rows, int32_t k, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream);
 ssmi_status ssmi_mx4_quantize_kernel(const void* w, int32_t k, int32_t n, int32_t dtype, uint8_t* codes, uint8_t* scales, void* stream);
 ssmi_status ssmi_mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int32_t k, int32_t n, float* w, void* stream);

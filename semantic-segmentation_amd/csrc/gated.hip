@@ -20,7 +20,7 @@ __device__ __forceinline__ float param_at(const void* p, int bf, int64_t i) {
 }
 
 // Stages, K step, q rows that the epilogue takes at once and workgroups to a CU (registers and LDS) of a tile shape.  The products of dx
-// and dW run long K loops: 128-byte steps, fewer barriers (16k x 512 -> 2048: dx 65 us, with 64-byte steps 92).  The gate kernels run
+// and dW run long K loops: 128-byte steps, fewer barriers (16k x 512 -> 2048 bfloat16: dx 147 us, with 64-byte steps 182).  The gate kernels run
 // short ones with an epilogue as long: the 128 x 128 tile takes 64-byte steps and a quarter of the tile through LDS at a time, so three
 // workgroups share a CU and one's epilogue runs under the others' products.
 template <int SP, int SQ>
@@ -159,9 +159,10 @@ __global__ __launch_bounds__(256, (gate_per_cu<T, SP, SQ, LONG>())) void gate_ke
       }
     };
     if constexpr (sizeof(T) == 2 && !BWD) {
-      // The forward pass stores straight from the accumulators: no LDS, no barrier, 32 bytes of a row at a time (64k x 512 -> 2048: 385 ->
-      // 371 us, 16k rows 83 -> 74).  Where dy has to come the same way, or nothing but the store is to do (dx), whole rows through LDS
-      // are faster (64k x 512 -> 2048 with dg, du: 421 against 476 us; 16k rows, dx: 66 against 72).
+      // The forward pass stores straight from the accumulators: no LDS, no barrier, 32 bytes of a row at a time (64k x 512 -> 2048: 306 us,
+      // through LDS 317, 16k rows 74 and 78).  Where dy has to come the same way, or nothing but the store is to do (dx), whole rows through
+      // LDS are faster (both measured with one bfloat16 term of dg and du: 64k x 512 -> 2048 with dg, du 421 against 476 us; 16k rows, dx 66
+      // against 72).
       if (whole && a.vec_out == 2) {
         const int hh = lane >> 5, u0 = wp * (SP / 2) * 32;
         T* const y = out + (int64_t)(s.wq * SQ * 32) * a.out_ld + u0;
@@ -468,7 +469,8 @@ __global__ __launch_bounds__(kReduce) void gate_reduce_kernel(ReduceArgs a) {
 }
 
 // memory rows brought to the tile engine's form: activation type, rows of cols_p >= cols values (16-byte multiples), zeros behind.
-// Up to three matrices a launch (x, both kernels), one per blockIdx.y.
+// Up to three matrices a launch (x, both kernels), one per blockIdx.y.  float32 kernels under bfloat16 rows become bfloat16 here, as the
+// convolutions' bfloat16 packs do: the matrix instructions take one type, and a second term would double the products of the forward pass.
 struct PadJob {
   const void* src;
   void* dst;
@@ -596,11 +598,12 @@ static_assert(past_rows<GateShape<2, 1>>(2) <= kPastRows && past_rows<GateShape<
               past_rows<ProductShape<2, 1>>(2) <= kPastRows && past_rows<ProductShape<2, 2>>(2) <= kPastRows && past_rows<ProductShape<2, 4>>(2) <= kPastRows, "");
 
 // Tile shapes (columns p x rows q), chosen by how many workgroups they make: a card of 256 CUs wants 512 of those that go two to a CU.
-//   gate: 128 x 256 where that makes 384 tiles, 128 x 128 where that makes 256, else 128 x 64
+//   gate: 128 x 256 where that makes 384 tiles (64k x 512 -> 2048 bfloat16: forward 301 us, with dg and du 464; 128 x 128 330 and 510), 128 x 128
+//         where that makes 256, else 128 x 64
 //   no tile of 128 rows or channels where there are 64 (131k x 64 -> 256 float32, dx 142 -> 103 us, dW 127 -> 90)
-//   dx:   256 x 256 (one to a CU: no epilogue to hide, 1115 TFLOP/s against 940 with 128 x 256) where that makes 192; 64 x 64 under 64 channels or where 128 x 64
-//         makes under 384 (4096 x 512 -> 2048 bfloat16 41 -> 36 us, 16k x 128 -> 512 float32 49 -> 47); else as above
-//   dW:   128 x 256 under strips of 4096 rows; else as above, counting the strips
+//   dx:   256 x 256 (one to a CU: no epilogue to hide; 64k x 512 -> 2048 bfloat16 477 us, 128 x 128 594) where that makes 192; 64 x 64 under 64
+//         channels or where 128 x 64 makes under 384 (4096 x 512 -> 2048 bfloat16 76 -> 69 us, 16k x 128 -> 512 float32 46 -> 44); else as above
+//   dW:   128 x 256 under strips of 4096 rows (64k x 512 -> 2048 bfloat16 538 us, 128 x 128 611); else as above, counting the strips
 // float32 takes no wide tiles: its 64-cycle matrix instructions leave LDS time to spare, and its sums take twice the registers.
 enum Tile { kTile64x64, kTile128x64, kTile128x128, kTile128x256, kTile256x256 };
 static Tile tile_for(int64_t q, int64_t p, bool wide, int64_t times = 1) {
@@ -621,8 +624,9 @@ static Tile tile_for_dw(int64_t rows, int64_t c, int64_t p, bool wide, int64_t m
 // K steps that a strip of dx takes.  Its smallest tiles may leave the card idle under a long K; strips bring one or two workgroups to a CU, of
 // four steps (256 bfloat16, 128 float32 values) at least.  By measurement a step takes a workgroup 0.4 us in bfloat16, two workgroups of a CU
 // side by side, and 0.85 in float32, where the matrix unit is full with one of them; the strips' sums and their reduction take 6.
-// Whole backward pass, one strip and so: 64 x 64 -> 4096 bfloat16 122 and 20 us, float32 205 and 25; 31 x 80 -> 944 42 and 17, 60 and 21;
-// dx alone, one strip and two, where they do not pay: 16k x 64 -> 256 bfloat16 6.5 and 14, 2048 x 512 -> 512 8.5 and 15, float32 17 and 20, 27 and 29.
+// Whole backward pass, one strip and so: 64 x 64 -> 4096 bfloat16 126 and 21 us, float32 205 and 26; 31 x 80 -> 944 43 and 18, 61 and 23;
+// 2048 x 512 -> 512 bfloat16 43.5 and 42.1.  dx alone, one strip and two, where they do not pay: 16k x 64 -> 256 bfloat16 11.5 and 14, float32
+// 16 and 19, 2048 x 512 -> 512 float32 27 and 28.
 static int dx_each(Tile t, int64_t rows, int64_t c, int steps, bool bf) {
   const int64_t tiles = ceil_div64(rows, 64) * ceil_div64(c, 64);
   int best = steps;
