@@ -81,7 +81,10 @@ class _GatedFn(torch.autograd.Function):
         if torch.is_grad_enabled():      # create_graph=True: what follows is not recorded
             raise RuntimeError("gated_feed_forward has no second derivative")
         wg, wu, bg, bu, *kept = ctx.saved_tensors
-        x = kept[0] if ctx.kept_as is None else Checkpoint8._made(*kept, *ctx.kept_as).restore()
+        wg, wu = _dense(wg), _dense(wu)      # saved-tensor hooks may give them back in another layout
+        if bg is not None:
+            bg, bu = bg.contiguous(), bu.contiguous()
+        x = kept[0] if ctx.kept_as is None else Checkpoint8(*kept, *ctx.kept_as).restore()
         nx, ng, nu, nbg, nbu = ctx.needs_input_grad[:5]
         c, f = wg.shape
         t, rows, ld = _aligned_rows(x)

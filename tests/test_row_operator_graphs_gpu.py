@@ -102,3 +102,19 @@ def test_restore_into_a_tensor_counts_as_a_change_of_it():
         assert torch.equal(kept.restore(out=w), buf)
     with torch.inference_mode():
         assert torch.equal(kept.restore(out=torch.zeros(6, 40, device=DEV)), buf)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "8bit"])
+def test_saved_tensors_may_come_back_in_another_layout(checkpoint):
+    """A hook gives back equal values; how they lie in memory is its own affair."""
+    args = tensors(c=48, grad=True)
+    want = torch.autograd.grad(ff.gated_feed_forward(*args, checkpoint=checkpoint).sum(), args)
+
+    def other(t):
+        return t.t().contiguous().t() if t.dim() == 2 else torch.stack([t, t], -1)[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(other, lambda t: t):
+        y = ff.gated_feed_forward(*args, checkpoint=checkpoint)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), args), want))
+    with torch.autograd.graph.save_on_cpu():
+        y = ff.gated_feed_forward(*args, checkpoint=checkpoint)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), args), want))
